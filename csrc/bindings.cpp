@@ -7,12 +7,14 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
+#include <algorithm>
 #include <cstring>
 #include <stdexcept>
 #include <string>
 #include <tuple>
 #include <vector>
 
+#include "expert_ops.h"
 #include "fused_tp.h"
 #include "gemm_sm100.h"
 #include "moe_a2a.h"
@@ -218,6 +220,96 @@ std::vector<SyncPage*> sync_list(const std::vector<uintptr_t>& v) {
   for (auto p : v) out.push_back(reinterpret_cast<SyncPage*>(p));
   return out;
 }
+
+// The tensors of one gradient-norm call, read from Python objects with the usual tensor methods (data_ptr, numel, dtype,
+// get_device, is_contiguous): a loop here costs a fraction of the same loop in Python, and some hundred tensors are ordinary.
+struct GradList {
+  std::vector<msccl::sm100::GradTensor> tensors;
+  int device = -1;
+
+  GradList(const py::list& grads, const py::object& outs, const py::tuple& dtypes, const py::function& same_dense_layout) {
+    const bool in_place = outs.is_none();
+    static PyObject* names[4] = {PyUnicode_InternFromString("data_ptr"), PyUnicode_InternFromString("numel"),
+                                 PyUnicode_InternFromString("get_device"), PyUnicode_InternFromString("is_contiguous")};
+    static PyObject* dtype_name = PyUnicode_InternFromString("dtype");
+    auto call = [&](PyObject* t, int which) {
+      PyObject* args[1] = {t};
+      PyObject* r = PyObject_VectorcallMethod(names[which], args, 1, nullptr);
+      if (r == nullptr) throw py::error_already_set();
+      return py::reinterpret_steal<py::object>(r);
+    };
+    auto elem_type = [&](PyObject* t, size_t i, const char* what) {
+      PyObject* d = PyObject_GetAttr(t, dtype_name);
+      if (d == nullptr) throw py::error_already_set();
+      const py::object dtype = py::reinterpret_steal<py::object>(d);
+      for (int k = 0; k < 3; ++k)
+        if (dtype.ptr() == PyTuple_GET_ITEM(dtypes.ptr(), k)) return static_cast<short>(k);
+      throw py::value_error(std::string(what) + " " + std::to_string(i) + " is not float32, bfloat16 or float16");
+    };
+    const py::list out_list = in_place ? py::list() : py::list(outs);
+    if (!in_place && out_list.size() != grads.size()) throw py::value_error("as many output tensors as gradients are needed");
+    tensors.reserve(grads.size());
+    for (size_t i = 0; i < grads.size(); ++i) {
+      PyObject* g = PyList_GET_ITEM(grads.ptr(), static_cast<Py_ssize_t>(i));
+      PyObject* o = in_place ? g : PyList_GET_ITEM(out_list.ptr(), static_cast<Py_ssize_t>(i));
+      msccl::sm100::GradTensor t;
+      std::memset(&t, 0, sizeof(t));
+      t.src_type = elem_type(g, i, "gradient");
+      t.dst_type = in_place ? t.src_type : elem_type(o, i, "output");
+      t.numel = PyLong_AsLongLong(call(g, 1).ptr());
+      bool plain = PyObject_IsTrue(call(g, 3).ptr()) == 1;
+      for (PyObject* x : {g, o}) {
+        const long dev = PyLong_AsLong(call(x, 2).ptr());
+        if (device < 0) device = static_cast<int>(dev);
+        if (dev < 0 || dev != device) throw py::value_error("tensor " + std::to_string(i) + " is not on the CUDA device of the others");
+        if (in_place) break;
+      }
+      if (!in_place) {
+        if (PyLong_AsLongLong(call(o, 1).ptr()) != t.numel) throw py::value_error("output " + std::to_string(i) + " has another size than its gradient");
+        plain = plain && PyObject_IsTrue(call(o, 3).ptr()) == 1;
+      }
+      if (!plain && !same_dense_layout(py::handle(g), py::handle(o)).cast<bool>())
+        throw py::value_error("gradient " + std::to_string(i) + " is not dense, or its output is laid out differently");
+      t.src = reinterpret_cast<const void*>(PyLong_AsUnsignedLongLong(call(g, 0).ptr()));
+      t.dst = in_place ? const_cast<void*>(t.src) : reinterpret_cast<void*>(PyLong_AsUnsignedLongLong(call(o, 0).ptr()));
+      if (PyErr_Occurred()) throw py::error_already_set();
+      if (t.numel > 0) tensors.push_back(t);
+    }
+  }
+
+  // Does any output share memory with another output, or with a gradient other than the one that it replaces?
+  bool overlapping() const {
+    static const int size[3] = {4, 2, 2};
+    struct Range { uintptr_t lo, hi; bool dst; };
+    std::vector<Range> r;
+    r.reserve(2 * tensors.size());
+    for (const auto& t : tensors) {
+      const uintptr_t s = reinterpret_cast<uintptr_t>(t.src), d = reinterpret_cast<uintptr_t>(t.dst);
+      r.push_back({d, d + t.numel * size[t.dst_type], true});
+      if (s != d || t.src_type != t.dst_type) r.push_back({s, s + t.numel * size[t.src_type], false});
+    }
+    std::sort(r.begin(), r.end(), [](const Range& a, const Range& b) { return a.lo < b.lo; });
+    uintptr_t dst_end = 0, src_end = 0;
+    for (const auto& x : r) {
+      if (x.lo < dst_end || (x.dst && x.lo < src_end)) return true;
+      uintptr_t& end = x.dst ? dst_end : src_end;
+      end = std::max(end, x.hi);
+    }
+    return false;
+  }
+
+  template <typename F>
+  void parts(F&& f) const {
+    for (size_t i = 0; i < tensors.size(); i += msccl::sm100::kGradTensorsPerLaunch)
+      f(tensors.data() + i, static_cast<int>(std::min<size_t>(tensors.size() - i, msccl::sm100::kGradTensorsPerLaunch)));
+  }
+
+  int partials() const {
+    int n = 0;
+    parts([&](const msccl::sm100::GradTensor* t, int count) { n += msccl::sm100::grad_norm_partials(t, count); });
+    return n;
+  }
+};
 
 }  // namespace
 
@@ -480,6 +572,75 @@ PYBIND11_MODULE(_msccl_native, m) {
   m.def("moe_sort", [](uintptr_t expert_of, int n, int experts, uintptr_t sorted_copy, uintptr_t expert_start, uintptr_t stream) {
     check_rt(msccl::sm100::launch_moe_sort(reinterpret_cast<const int*>(expert_of), n, experts, reinterpret_cast<int*>(sorted_copy),
                                            reinterpret_cast<int*>(expert_start), as_stream(stream)), "launch of the MoE sort kernel");
+  });
+  // Rows around the experts: elem 0 = fp32, 1 = bf16, 2 = fp16; pointers that may be 0 are said to be in moe_rows.cu.
+  m.def("sort_copies", [](uintptr_t expert_of, bool wide_ids, long long n, int experts, uintptr_t sorted_copy, uintptr_t expert_start,
+                          uintptr_t position, uintptr_t stream) {
+    check_rt(msccl::sm100::launch_sort_copies(reinterpret_cast<const void*>(expert_of), wide_ids, n, experts, reinterpret_cast<int*>(sorted_copy),
+                                              reinterpret_cast<int*>(expert_start), reinterpret_cast<int*>(position), as_stream(stream)),
+             "launch of the copy sort kernel");
+  });
+  m.def("scatter_rows", [](uintptr_t x, long long ldx, uintptr_t out, uintptr_t position, uintptr_t rows_kept, int tokens, int topk, int hidden,
+                           int elem, uintptr_t stream) {
+    check_rt(msccl::sm100::launch_scatter_rows(reinterpret_cast<const void*>(x), ldx, reinterpret_cast<void*>(out),
+                                               reinterpret_cast<const int*>(position), reinterpret_cast<const int*>(rows_kept), tokens, topk,
+                                               hidden, elem, as_stream(stream)),
+             "launch of the row scatter kernel");
+  });
+  m.def("combine_rows", [](uintptr_t ys, long long ldy, uintptr_t weights, uintptr_t out, uintptr_t position, uintptr_t rows_kept, int tokens,
+                           int topk, int hidden, int elem, uintptr_t stream) {
+    check_rt(msccl::sm100::launch_combine_rows(reinterpret_cast<const void*>(ys), ldy, reinterpret_cast<const float*>(weights),
+                                               reinterpret_cast<void*>(out), reinterpret_cast<const int*>(position),
+                                               reinterpret_cast<const int*>(rows_kept), tokens, topk, hidden, elem, as_stream(stream)),
+             "launch of the row combine kernel");
+  });
+  m.def("combine_backward", [](uintptr_t dy, long long lddy, uintptr_t ys, long long ldy, uintptr_t weights, uintptr_t dys, uintptr_t dweights,
+                               uintptr_t position, uintptr_t rows_kept, int tokens, int topk, int hidden, int elem, uintptr_t stream) {
+    check_rt(msccl::sm100::launch_combine_backward(reinterpret_cast<const void*>(dy), lddy, reinterpret_cast<const void*>(ys), ldy,
+                                                   reinterpret_cast<const float*>(weights), reinterpret_cast<void*>(dys),
+                                                   reinterpret_cast<float*>(dweights), reinterpret_cast<const int*>(position),
+                                                   reinterpret_cast<const int*>(rows_kept), tokens, topk, hidden, elem, as_stream(stream)),
+             "launch of the combine gradient kernel");
+  });
+  // Products of the rows of every group with the group's matrix, and the gradient of the matrices.
+  m.def("grouped_gemm", [](uintptr_t x, long long ldx, uintptr_t w, long long ldw, long long lde, uintptr_t offsets, uintptr_t out, long long ldo,
+                           int rows, int groups, int n, int k, bool backward, int elem, int bn, bool zero_rest, uintptr_t error_words,
+                           uintptr_t stream) {
+    check_rt(msccl::sm100::launch_grouped_gemm(reinterpret_cast<const void*>(x), ldx, reinterpret_cast<const void*>(w), ldw, lde,
+                                               reinterpret_cast<const int*>(offsets), reinterpret_cast<void*>(out), ldo, rows, groups, n, k,
+                                               backward, elem, bn, zero_rest, reinterpret_cast<int*>(error_words), as_stream(stream)),
+             "launch of the grouped GEMM kernel");
+  });
+  m.def("grouped_wgrad", [](uintptr_t dy, long long lddy, uintptr_t x, long long ldx, uintptr_t offsets, uintptr_t out, long long ldo, long long lde,
+                            int rows, int groups, int n, int k, int elem, bool f32_out, uintptr_t error_words, uintptr_t stream) {
+    check_rt(msccl::sm100::launch_grouped_wgrad(reinterpret_cast<const void*>(dy), lddy, reinterpret_cast<const void*>(x), ldx,
+                                                reinterpret_cast<const int*>(offsets), reinterpret_cast<void*>(out), ldo, lde, rows, groups, n,
+                                                k, elem, f32_out, reinterpret_cast<int*>(error_words), as_stream(stream)),
+             "launch of the grouped weight gradient kernel");
+  });
+  // Gradient norm and clipping of a list of tensors (grad_norm.cu).
+  py::class_<GradList>(m, "GradList")
+      .def(py::init<const py::list&, const py::object&, const py::tuple&, const py::function&>())
+      .def_readonly("device", &GradList::device)
+      .def("__len__", [](const GradList& g) { return g.tensors.size(); })
+      .def("overlapping", &GradList::overlapping)
+      .def("partials", &GradList::partials);
+  m.def("grad_norm", [](const GradList& g, uintptr_t partials, uintptr_t stream) {
+    double* p = reinterpret_cast<double*>(partials);
+    g.parts([&](const msccl::sm100::GradTensor* t, int count) {
+      check_rt(msccl::sm100::launch_grad_norm(t, count, p, as_stream(stream)), "launch of the gradient norm kernel");
+      p += msccl::sm100::grad_norm_partials(t, count);
+    });
+  });
+  m.def("grad_sum", [](uintptr_t partials, int count, uintptr_t sum, uintptr_t norm, uintptr_t stream) {
+    check_rt(msccl::sm100::launch_grad_sum(reinterpret_cast<const double*>(partials), count, reinterpret_cast<double*>(sum),
+                                           reinterpret_cast<float*>(norm), as_stream(stream)), "launch of the gradient sum kernel");
+  });
+  m.def("grad_scale", [](const GradList& g, uintptr_t partials, int count, double max_norm, uintptr_t norm, uintptr_t stream) {
+    g.parts([&](const msccl::sm100::GradTensor* t, int n) {
+      check_rt(msccl::sm100::launch_grad_scale(t, n, reinterpret_cast<const double*>(partials), count, max_norm, reinterpret_cast<float*>(norm),
+                                               as_stream(stream)), "launch of the gradient scaling kernel");
+    });
   });
   // In-place all-reduce of `bytes` at `offset` of every rank's symmetric heap.  mc_base = 0
   // selects peer loads/stores, otherwise the NVLink multicast window is used.

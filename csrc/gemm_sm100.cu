@@ -283,6 +283,23 @@ CUtensorMap make_block512_map(const void* base, uint64_t blocks) {
   return map;
 }
 
+// Tensor map of 8- or 16-bit elements in two or three dimensions, 128-byte swizzle, zeros outside.
+CUtensorMap make_swizzled_map(const void* base, int elem_bytes, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+  CUtensorMap map;
+  cuuint64_t d[3], st[2];
+  cuuint32_t bx[3], es[3] = {1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+    if (i > 0) st[i - 1] = strides[i - 1];
+  }
+  const CUresult r = encode_fn()(&map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, static_cast<cuuint32_t>(rank),
+                                 const_cast<void*>(base), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed with code " + std::to_string(static_cast<int>(r)));
+  return map;
+}
+
 int sm_count() {
   static int count = 0;
   if (count == 0) {

@@ -1,0 +1,110 @@
+// Pieces shared by the grouped products (grouped_gemm.cu, grouped_wgrad.cu, fp8_block_gemm.cu): the table of groups, tensor maps of
+// two and three dimensions, descriptors of operands whose reduction dimension is not the contiguous one.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "gemm_sm100.cuh"
+#include "umma_2cta.cuh"
+
+namespace msccl {
+namespace sm100 {
+
+constexpr int kMaxGroups = 512;
+constexpr unsigned int kFullMask = 0xffffffffu;
+
+// Rows of every group and the number of tiles before it.  Offsets come from the device and may be anything: they are clamped to
+// [0, rows] and to their running maximum, so that groups never overlap and no index leaves the tensors.
+struct GroupTable {
+  int row_start[kMaxGroups + 1];
+  int tile_start[kMaxGroups + 1];
+};
+
+// Whole warp.  tiles_of(rows) = tiles of a group of that many rows.
+template <typename TilesOf>
+__device__ __forceinline__ void build_groups(GroupTable& g, const int* __restrict__ offsets, int groups, int rows, TilesOf tiles_of) {
+  const int lane = threadIdx.x % 32;
+  int high = 0;                                  // running maximum
+  for (int b = 0; b <= groups; b += 32) {
+    int v = b + lane <= groups ? min(max(offsets[b + lane], 0), rows) : 0;
+    v = max(v, high);
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int up = __shfl_up_sync(kFullMask, v, off);
+      if (lane >= off) v = max(v, up);
+    }
+    if (b + lane <= groups) g.row_start[b + lane] = v;
+    high = __shfl_sync(kFullMask, v, 31);
+  }
+  __syncwarp();
+  int before = 0;
+  if (lane == 0) g.tile_start[0] = 0;
+  for (int b = 0; b < groups; b += 32) {
+    int t = b + lane < groups ? tiles_of(g.row_start[b + lane + 1] - g.row_start[b + lane]) : 0;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int up = __shfl_up_sync(kFullMask, t, off);
+      if (lane >= off) t += up;
+    }
+    if (b + lane < groups) g.tile_start[b + lane + 1] = before + t;
+    before += __shfl_sync(kFullMask, t, 31);
+  }
+  __syncwarp();
+}
+
+// Loads of one CTA of a pair whose bytes are counted on the mbarrier at `bar`, which may belong to the partner (no multicast).
+__device__ __forceinline__ void tma_pair_2d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tma_pair_3d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
+// Operand whose M (or N) dimension is the contiguous one, 128-byte swizzle: slabs of 64 elements x 64 reduction rows (8 KB, 128
+// bytes per reduction row).  Leading byte offset: from one slab to the next; stride byte offset: 8 reduction rows.
+constexpr int kSlabBytes = 64 * 128;
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFF);
+  d |= static_cast<uint64_t>(kSlabBytes >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+// Bits of the instruction descriptor (kind::f16): fp32 accumulator, both operands f16 or both bf16.
+constexpr uint32_t kIdescTransA = 1u << 15, kIdescTransB = 1u << 16;
+__host__ __device__ constexpr uint32_t idesc_16bit(bool bf16, int m, int n) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+__device__ __forceinline__ uint32_t pack_16bit(bool bf16, float lo, float hi) {
+  uint32_t r;
+  if (bf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// A producer that gave up lets the loads that it issued land before shared memory is released (they take microseconds).
+__device__ __forceinline__ void drain_wait() {
+  unsigned long long t0, t1;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  do { asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1)); } while (t1 - t0 < 200000ull);
+}
+
+// Tensor maps (gemm_sm100.cu).  dims and box innermost first; strides in bytes, of dimensions 1 and up.
+CUtensorMap make_swizzled_map(const void* base, int elem_bytes, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box);
+
+}  // namespace sm100
+}  // namespace msccl

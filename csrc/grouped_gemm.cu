@@ -1,0 +1,321 @@
+// Products of the rows of every group with the group's matrix, for sm_100a:
+//
+//   forward    y[t, n]  = sum_k x[t, k]  w[e, n, k]        (w K-major: the reduction dimension is the contiguous one)
+//   backward   dx[t, k] = sum_n dy[t, n] w[e, n, k]        (w MN-major: read through descriptors, no transposed copy)
+//
+// for the rows t of group e, [offsets[e], offsets[e + 1]).  bf16 or fp16 in and out, fp32 accumulators.  Group sizes are known on
+// the device only: every CTA derives the same list of tiles from the offsets, so nothing is copied to the host.
+//
+// The weights are the M operand and the rows of the group the N operand of the MMA: 256 features (of a CTA pair, cta_group::2)
+// by BN rows.  The last tile of a group is then padded to a multiple of BN = 32 .. 256 rows instead of 256, and a decode batch
+// streams the weights through tiles of 32 rows.  Rows of a tile that belong to the next group only reach columns of the accumulator
+// that are not stored, whatever they hold.  What is left of both operands behind the reduction dimension reads as zero.
+//
+// The accumulator holds a feature per lane and a row per column; the epilogue transposes 8 x 8 values among eight lanes with shuffles,
+// so that a lane stores 16 bytes of one row and four lanes store 64 consecutive bytes.
+//
+// Synchronisation is that of gemm_2cta_sm100.cu.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <stdexcept>
+
+#include "expert_ops.h"
+#include "gemm_sm100.cuh"
+#include "gemm_sm100.h"
+#include "grouped_common.cuh"
+#include "umma_2cta.cuh"
+
+namespace msccl {
+namespace sm100 {
+
+namespace {
+
+constexpr int kGroupTileRows = 2048;             // rows that a group of tiles walks together (L2, see tile_coords)
+constexpr int kGABytes = BM * BK * 2;            // this CTA's 128 features: 16 KB
+constexpr int kGSmemLimit = 220 * 1024;
+
+template <int BN> struct Geometry {
+  static constexpr int kBBytes = BN / 2 * BK * 2;
+  static constexpr int kStageBytes = kGABytes + kBBytes;
+  static constexpr int kFit = (kGSmemLimit - 2048) / kStageBytes;
+  static constexpr int kStages = kFit < 10 ? kFit : 10;
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStageBytes + 256;
+  static constexpr int kTmemCols = 2 * BN;
+};
+
+struct GroupedArgs {
+  const int* offsets;
+  uint16_t* out;
+  long long ldo;
+  int rows, groups, features, reduction;
+  int zero_rest;                                 // rows of no group become zero
+  int* error_words;
+};
+
+template <int BN, bool MN_MAJOR, bool BF16>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const GroupedArgs g) {
+  using Geo = Geometry<BN>;
+  constexpr int S = Geo::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ GroupTable table;
+  __shared__ int s_skip;
+  uint8_t* stage_base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stage_base + static_cast<size_t>(S) * Geo::kStageBytes);
+  uint64_t *full_bar = bars, *empty_bar = bars + S, *acc_full = bars + 2 * S, *acc_empty = bars + 2 * S + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int f_tiles = (g.features + 2 * BM - 1) / (2 * BM);
+  const int k_blocks = (g.reduction + BK - 1) / BK;
+  const int first = static_cast<int>(cluster_id_x()), step = static_cast<int>(num_clusters_x());
+
+  if (threadIdx.x == 0) {
+    // an earlier launch gave up: skip the work; the leader's reading decides for the pair
+    s_skip = g.error_words != nullptr && *reinterpret_cast<volatile int*>(g.error_words) != 0 ? 1 : 0;
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 8);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+    prefetch_tensormap(&map_w);
+    prefetch_tensormap(&map_x);
+  }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, Geo::kTmemCols);
+  if (warp == 2) build_groups(table, g.offsets, g.groups, g.rows, [&](int rows) { return (rows + BN - 1) / BN * f_tiles; });
+  tc_fence_before_sync();
+  cluster_sync_all();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  const bool skip = ld_shared_cluster_u32(map_to_cta(smem_u32(&s_skip), 0)) != 0;
+  const int num_tiles = table.tile_start[g.groups];
+
+  // tile -> group e, first row and first feature; e only moves forward
+  auto locate = [&](int tile, int& e, int& row, int& feature) {
+    while (tile >= table.tile_start[e + 1]) ++e;
+    const int rows = table.row_start[e + 1] - table.row_start[e];
+    int tm, tn;
+    tile_coords(tile - table.tile_start[e], (rows + BN - 1) / BN, f_tiles, kGroupTileRows / BN, tm, tn);
+    row = table.row_start[e] + tm * BN;
+    feature = tn * 2 * BM;
+  };
+
+  if (skip) {
+    // fall through to the common exit
+  } else if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0, e = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = first; tile < num_tiles && ok; tile += step) {
+        int row, feature;
+        locate(tile, e, row, feature);
+        row += static_cast<int>(rank) * (BN / 2);
+        feature += static_cast<int>(rank) * BM;
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) {
+            gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_EMPTY, 0, stage);
+            ok = false;
+            break;
+          }
+          uint8_t* a_dst = stage_base + static_cast<size_t>(stage) * Geo::kStageBytes;
+          if (leader) mbar_expect_tx(&full_bar[stage], 2 * Geo::kStageBytes);
+          const uint32_t bar = map_to_cta(smem_u32(&full_bar[stage]), 0);
+          if (MN_MAJOR) {
+            tma_pair_3d(a_dst, &map_w, bar, feature, kb * BK, e);
+            tma_pair_3d(a_dst + kSlabBytes, &map_w, bar, feature + 64, kb * BK, e);
+          } else {
+            tma_pair_3d(a_dst, &map_w, bar, kb * BK, feature, e);
+          }
+          tma_pair_2d(a_dst + kGABytes, &map_x, bar, kb * BK, row);
+          if (++stage == S) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok) drain_wait();
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      constexpr uint32_t idesc = idesc_16bit(BF16, 2 * BM, BN) | (MN_MAJOR ? kIdescTransA : 0u);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int tile = first; tile < num_tiles && ok; tile += step) {
+        if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1, abort_flag)) {
+          gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 1, acc);
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * BN);
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, abort_flag)) {
+            gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_FULL, 1, stage);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t a_addr = smem_u32(stage_base + static_cast<size_t>(stage) * Geo::kStageBytes);
+          const uint64_t adesc = MN_MAJOR ? smem_desc_mn_sw128(a_addr) : smem_desc_sw128(a_addr);
+          const uint64_t bdesc = smem_desc_sw128(a_addr + kGABytes);
+          constexpr uint64_t a_step = MN_MAJOR ? 16 * 128 / 16 : 2;      // 16 reduction elements, in units of 16 bytes
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k)
+            umma_bf16_pair(tmem_d, adesc + k * a_step, bdesc + static_cast<uint64_t>(k * 2), idesc, (kb | k) != 0);
+          tc_commit_pair(&empty_bar[stage], 3);
+          if (++stage == S) { stage = 0; phase ^= 1; }
+        }
+        if (ok) tc_commit_pair(&acc_full[acc], 3);
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      }
+    }
+  } else {
+    const int quarter = warp % 4;
+    int acc = 0, e = 0;
+    uint32_t acc_phase = 0;
+    for (int tile = first; tile < num_tiles; tile += step) {
+      int row, feature;
+      locate(tile, e, row, feature);
+      const int row_end = table.row_start[e + 1];
+      bool ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag);
+      ok = __all_sync(kFullMask, ok);
+      if (!ok) {
+        if (lane == 0) gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 2, acc);
+        break;
+      }
+      tc_fence_after_sync();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BN);
+      const int f = feature + static_cast<int>(rank) * BM + quarter * 32 + (lane & ~7);       // this lane stores features f .. f + 7
+      const bool in = f < g.features;
+      const int columns = min(BN, row_end - row);
+      for (int c = 0; c < columns; c += 32) {
+        uint32_t r[32];
+        tmem_ld32(taddr + c, r);
+        tc_wait_ld();
+        // 1: (feature pair, row 2 i + bit 0 of the lane)
+        uint32_t s[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t p = pack_16bit(BF16, __uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+          const uint32_t q = __shfl_xor_sync(kFullMask, p, 1);
+          s[i] = (lane & 1) ? __byte_perm(q, p, 0x7632) : __byte_perm(p, q, 0x5410);
+        }
+        // 2: four features, row 4 j + two bits of the lane
+        uint2 u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool up = (lane & 2) != 0;
+          const uint32_t got = __shfl_xor_sync(kFullMask, up ? s[2 * j] : s[2 * j + 1], 2);
+          u[j] = up ? make_uint2(got, s[2 * j + 1]) : make_uint2(s[2 * j], got);
+        }
+        // 3: eight features, row 8 m + three bits of the lane
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const bool up = (lane & 4) != 0;
+          const uint2 give = up ? u[2 * m] : u[2 * m + 1];
+          const uint2 got = make_uint2(__shfl_xor_sync(kFullMask, give.x, 4), __shfl_xor_sync(kFullMask, give.y, 4));
+          const uint4 v = up ? make_uint4(got.x, got.y, u[2 * m + 1].x, u[2 * m + 1].y) : make_uint4(u[2 * m].x, u[2 * m].y, got.x, got.y);
+          const int t = c + 8 * m + (lane & 7);
+          if (in && t < columns) *reinterpret_cast<uint4*>(g.out + (row + t) * g.ldo + f) = v;
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[acc]), 0));
+      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+    }
+    if (g.zero_rest) {                           // rows before the first group and behind the last one
+      const int head = table.row_start[0], tail = table.row_start[g.groups];
+      const int rest = head + g.rows - tail;
+      for (int i = blockIdx.x * 4 + quarter; i < rest; i += gridDim.x * 4) {
+        uint4* dst = reinterpret_cast<uint4*>(g.out + static_cast<long long>(i < head ? i : tail + i - head) * g.ldo);
+        for (int v = lane; v < g.features / 8; v += 32) dst[v] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+
+  tc_fence_before_sync();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, Geo::kTmemCols);
+  }
+}
+
+template <int BN, bool MN_MAJOR, bool BF16>
+cudaError_t launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const GroupedArgs& g, int most_tiles, cudaStream_t stream) {
+  static int cached[64] = {};
+  auto kernel = grouped_gemm_kernel<BN, MN_MAJOR, BF16>;
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (cached[dev] == 0) {
+    int clusters = 0;
+    err = pair_clusters(kernel, Geometry<BN>::kSmem, &clusters);
+    if (err != cudaSuccess) return err;
+    if (clusters <= 0) return cudaErrorLaunchOutOfResources;
+    cached[dev] = clusters;
+  }
+  return launch_pairs(kernel, Geometry<BN>::kSmem, most_tiles < cached[dev] ? most_tiles : cached[dev], stream, map_w, map_x, g);
+}
+
+template <int BN>
+cudaError_t launch_by_type(bool mn_major, bool bf16, const CUtensorMap& map_w, const CUtensorMap& map_x, const GroupedArgs& g, int most_tiles,
+                           cudaStream_t stream) {
+  if (mn_major) return bf16 ? launch<BN, true, true>(map_w, map_x, g, most_tiles, stream) : launch<BN, true, false>(map_w, map_x, g, most_tiles, stream);
+  return bf16 ? launch<BN, false, true>(map_w, map_x, g, most_tiles, stream) : launch<BN, false, false>(map_w, map_x, g, most_tiles, stream);
+}
+
+}  // namespace
+
+// w: [groups, n, k] (pitch ldw, matrix stride lde, elements); x: [rows, k] and out: [rows, n], or with `backward` x: [rows, n]
+// (dy) and out: [rows, k].  n % 8 == 0, k % 8 == 0, everything 16-byte aligned.  bn: 32, 64, 128 or 256 rows per tile.
+cudaError_t launch_grouped_gemm(const void* x, long long ldx, const void* w, long long ldw, long long lde, const int* offsets, void* out,
+                                long long ldo, int rows, int groups, int n, int k, bool backward, int elem, int bn, bool zero_rest,
+                                int* error_words, cudaStream_t stream) {
+  if (rows < 1 || groups < 1 || groups > kMaxGroups || n < 8 || k < 8 || n % 8 != 0 || k % 8 != 0 || ldx % 8 != 0 || ldw % 8 != 0 ||
+      lde % 8 != 0 || ldo % 8 != 0 || (elem != kElemBF16 && elem != kElemF16))
+    return cudaErrorInvalidValue;
+  GroupedArgs g;
+  g.offsets = offsets;
+  g.out = static_cast<uint16_t*>(out);
+  g.ldo = ldo;
+  g.rows = rows;
+  g.groups = groups;
+  g.features = backward ? k : n;
+  g.reduction = backward ? n : k;
+  g.zero_rest = zero_rest ? 1 : 0;
+  g.error_words = error_words;
+  const uint64_t w_dims[3] = {static_cast<uint64_t>(k), static_cast<uint64_t>(n), static_cast<uint64_t>(groups)};
+  const uint64_t w_strides[2] = {static_cast<uint64_t>(ldw) * 2, static_cast<uint64_t>(lde) * 2};
+  const uint32_t w_box[3] = {64, backward ? 64u : 128u, 1};
+  const CUtensorMap map_w = make_swizzled_map(w, 2, 3, w_dims, w_strides, w_box);
+  const uint64_t x_dims[2] = {static_cast<uint64_t>(g.reduction), static_cast<uint64_t>(rows)};
+  const uint64_t x_strides[1] = {static_cast<uint64_t>(ldx) * 2};
+  const uint32_t x_box[2] = {64, static_cast<uint32_t>(bn / 2)};
+  const CUtensorMap map_x = make_swizzled_map(x, 2, 2, x_dims, x_strides, x_box);
+  // as many tiles as there can be: every group may end inside one
+  const long long f_tiles = (g.features + 2 * BM - 1) / (2 * BM), active = groups < rows ? groups : rows;
+  const long long most = f_tiles * (rows / bn + active);
+  if (most > (1ll << 30)) return cudaErrorInvalidValue;
+  const int most_tiles = most < 1 ? 1 : static_cast<int>(most);
+  const bool bf16 = elem == kElemBF16;
+  switch (bn) {
+    case 32: return launch_by_type<32>(backward, bf16, map_w, map_x, g, most_tiles, stream);
+    case 64: return launch_by_type<64>(backward, bf16, map_w, map_x, g, most_tiles, stream);
+    case 128: return launch_by_type<128>(backward, bf16, map_w, map_x, g, most_tiles, stream);
+    case 256: return launch_by_type<256>(backward, bf16, map_w, map_x, g, most_tiles, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace sm100
+}  // namespace msccl

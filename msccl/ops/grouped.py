@@ -1,0 +1,121 @@
+"""Matrix products grouped by expert with ragged sizes: the rows of expert ``e`` (``offsets[e] .. offsets[e + 1]`` of a row-sorted
+matrix, as ``sort_copies`` gives them) times that expert's weights, forward and both gradients (``csrc/grouped_gemm.cu``,
+``csrc/grouped_wgrad.cu``).  Any number of rows per expert, none included; there is no capacity and no padding.
+
+``offsets`` [experts + 1] int32 stays on the device: no call waits for it.  Values are clamped to the rows and to their running
+maximum.  Rows that belong to no expert come out as zeros, or, in an ``out`` that the caller gives, are left as they were.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from msccl.ops._launch import (ELEMS, check, check_apart, check_devices, check_matrix, check_offsets, error_words, on_stream, pitch,
+                               stream_handle)
+from msccl.ops.moe_rows import MAX_EXPERTS, _kernel_rows
+from msccl.runtime.native import load
+
+_TYPES = (torch.bfloat16, torch.float16)
+
+
+def _tile_rows(rows, experts):
+    mean = rows / max(1, min(rows, experts))
+    return 32 if mean <= 32 else 64 if mean <= 64 else 128 if mean <= 768 else 256
+
+
+def _check_experts(experts):
+    check(1 <= experts <= MAX_EXPERTS, f'between 1 and {MAX_EXPERTS} experts are supported (got {experts})')
+
+
+def _product(x, w, offsets, out, backward):
+    experts, n, k = w.shape
+    columns = k if backward else n
+    given = out is not None
+    if not given:
+        out = torch.empty(x.shape[0], columns, dtype=x.dtype, device=x.device)
+    if x.shape[0]:
+        load().grouped_gemm(x.data_ptr(), pitch(x), w.data_ptr(), pitch(w), w.stride(0) if experts > 1 else n * pitch(w), offsets.data_ptr(),
+                            out.data_ptr(), pitch(out), x.shape[0], experts, n, k, backward, ELEMS[x.dtype],
+                            _tile_rows(x.shape[0], experts), not given, error_words(x.device), stream_handle())
+    return out
+
+
+def _weight_gradient(dy, x, offsets, out=None, dtype=None):
+    experts, n, k = offsets.numel() - 1, dy.shape[1], x.shape[1]
+    if out is None:
+        out = torch.empty(experts, n, k, dtype=dtype or x.dtype, device=x.device)
+    if x.shape[0] == 0:
+        return out.zero_()
+    load().grouped_wgrad(dy.data_ptr(), pitch(dy), x.data_ptr(), pitch(x), offsets.data_ptr(), out.data_ptr(), pitch(out),
+                         out.stride(0) if experts > 1 else n * pitch(out), x.shape[0], experts, n, k, ELEMS[x.dtype],
+                         out.dtype == torch.float32, error_words(x.device), stream_handle())
+    return out
+
+
+class _Grouped(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, offsets):
+        ctx.save_for_backward(x, w, offsets)
+        return _product(x, w, offsets, None, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w, offsets = ctx.saved_tensors
+        with on_stream(dy.device, None):
+            dy = _kernel_rows(dy, x.dtype)
+            dx = _product(dy, w, offsets, None, True) if ctx.needs_input_grad[0] else None
+            dw = _weight_gradient(dy, x, offsets) if ctx.needs_input_grad[1] else None
+        return dx, dw, None
+
+
+def _check_product(x, name, w, offsets, out, backward):
+    check_matrix(w, 'w', _TYPES, 8, dims=3)
+    experts, n, k = w.shape
+    width, columns = (n, k) if backward else (k, n)
+    _check_experts(experts)
+    check(n > 0 and n % 8 == 0, f'both dimensions of a weight must be positive multiples of 8 (got {n})')
+    check_matrix(x, name, (w.dtype,), 8)
+    check(x.shape[1] == width, f'{name} has {x.shape[1]} columns, the weights expect {width}')
+    check_offsets(offsets, experts)
+    if out is not None:
+        check_matrix(out, 'out', (w.dtype,), 8)
+        check(out.shape == (x.shape[0], columns), f'out must be [{x.shape[0]}, {columns}] (got {list(out.shape)})')
+        check_apart(out, **{name: x, 'w': w})
+    return check_devices(**{name: x, 'w': w, 'offsets': offsets, 'out': out})
+
+
+def grouped_gemm(x, w, offsets, out=None, stream=None):
+    """``y[t] = w[e] @ x[t]`` for the rows ``t`` of every expert ``e``: ``x`` [rows, k], ``w`` [experts, n, k] (both bf16 or both fp16,
+    n and k multiples of 8, rows contiguous), result [rows, n] of the same type, fp32 sums.  Differentiable in ``x`` and ``w``; with
+    ``out`` the result has no gradient."""
+    device = _check_product(x, 'x', w, offsets, out, False)
+    needs = torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
+    check(out is None or not needs, 'a result written to out has no gradient: detach x and w, or leave out away')
+    with on_stream(device, stream, x, w, offsets, *(() if out is None else (out,))):
+        return _Grouped.apply(x, w, offsets) if needs else _product(x, w, offsets, out, False)
+
+
+def grouped_gemm_dgrad(dy, w, offsets, out=None, stream=None):
+    """``dx[t] = w[e].T @ dy[t]``: ``dy`` [rows, n], ``w`` [experts, n, k], result [rows, k].  No gradient of its own."""
+    device = _check_product(dy, 'dy', w, offsets, out, True)
+    with on_stream(device, stream, dy, w, offsets, *(() if out is None else (out,))), torch.no_grad():
+        return _product(dy, w, offsets, out, True)
+
+
+def grouped_gemm_wgrad(dy, x, offsets, out=None, dtype=None, stream=None):
+    """``dw[e] = sum of outer(dy[t], x[t])`` over the rows of expert ``e`` (zeros where it has none): ``dy`` [rows, n], ``x``
+    [rows, k], result [experts, n, k] of their type or, with ``dtype=torch.float32`` (or such an ``out``), the fp32 sums."""
+    check_matrix(x, 'x', _TYPES, 8)
+    check_matrix(dy, 'dy', (x.dtype,), 8)
+    check(x.shape[0] == dy.shape[0], f'dy has {dy.shape[0]} rows, x {x.shape[0]}')
+    experts = offsets.numel() - 1
+    _check_experts(experts)
+    check_offsets(offsets, experts)
+    check(dtype in (None, x.dtype, torch.float32), f'the gradient is {x.dtype} or float32 (asked for {dtype})')
+    if out is not None:
+        check_matrix(out, 'out', (x.dtype, torch.float32), 8, dims=3)
+        check(out.shape == (experts, dy.shape[1], x.shape[1]) and dtype in (None, out.dtype),
+              f'out must be [{experts}, {dy.shape[1]}, {x.shape[1]}] of the type asked for')
+        check_apart(out, dy=dy, x=x)
+    device = check_devices(dy=dy, x=x, offsets=offsets, out=out)
+    with on_stream(device, stream, dy, x, offsets, *(() if out is None else (out,))), torch.no_grad():
+        return _weight_gradient(dy, x, offsets, out, dtype)

@@ -1,0 +1,140 @@
+"""Rows around the experts of a MoE layer on one GPU: token copies sorted by expert, their rows gathered, the experts' results
+combined (``csrc/moe_rows.cu``).  Unlike ``FusedMoE``, which exchanges rows between GPUs inside its GEMM kernels, there is no
+capacity, and ``gather_rows`` and ``combine_rows`` have gradients.
+
+    order = sort_copies(experts, num_experts)             # experts [tokens, k], as the router chose them
+    xs = gather_rows(x, order)                            # [tokens * k, hidden], rows of expert e: order.offsets[e] .. [e + 1]
+    ys = grouped_gemm(xs, w, order.offsets)
+    y = combine_rows(ys, weights, order)                  # y[t] = sum_j weights[t, j] * (result of copy j of token t)
+"""
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from msccl.ops._launch import ELEMS, check, check_devices, check_matrix, on_stream, pitch, stream_handle
+from msccl.runtime.native import load
+
+MAX_EXPERTS, MAX_TOPK, MAX_COPIES = 512, 8, 1 << 22
+
+
+class CopyOrder(NamedTuple):
+    """``sorted_copy`` [tokens * k] int32: copies (``token * k + j``) ordered by expert, equal ones by number, dropped ones last.
+    ``offsets`` [num_experts + 1] int32: the rows of each expert; rows from ``offsets[-1]`` on belong to dropped copies.
+    ``position`` [tokens, k] int32: the row of each copy.  The tensors are made by ``sort_copies`` and are not to be changed."""
+    sorted_copy: torch.Tensor
+    offsets: torch.Tensor
+    position: torch.Tensor
+
+
+def sort_copies(experts, num_experts, stream=None):
+    """Stable order of the copies ``experts`` [tokens, k] (int32 or int64) by expert, in one launch.  A copy whose id is outside
+    ``[0, num_experts)`` is dropped: the gather gives it a row of zeros behind the last expert's, the combination ignores it."""
+    check(experts.dim() == 2 and experts.dtype in (torch.int32, torch.int64), 'experts must be a [tokens, k] int32 or int64 tensor')
+    tokens, topk = experts.shape
+    check(tokens >= 1 and 1 <= topk <= MAX_TOPK and tokens * topk <= MAX_COPIES,
+          f'sort_copies needs at least one token, k <= {MAX_TOPK} and at most {MAX_COPIES} copies (got {tokens} x {topk})')
+    check(1 <= num_experts <= MAX_EXPERTS, f'num_experts must be within 1 and {MAX_EXPERTS} (got {num_experts})')
+    with on_stream(check_devices(experts=experts), stream, experts):
+        experts = experts.contiguous()
+        copies = tokens * topk
+        table = torch.empty(2 * copies + num_experts + 1, dtype=torch.int32, device=experts.device)
+        sorted_copy, position, offsets = table[:copies], table[copies:2 * copies], table[2 * copies:]
+        load().sort_copies(experts.data_ptr(), experts.dtype == torch.int64, copies, num_experts, sorted_copy.data_ptr(),
+                           offsets.data_ptr(), position.data_ptr(), stream_handle())
+    return CopyOrder(sorted_copy, offsets, position.view(tokens, topk))
+
+
+def _check_rows(t, name):
+    check_matrix(t, name, ELEMS, 16 // t.element_size())
+
+
+def _rows_kept(order):
+    return order.offsets.data_ptr() + 4 * (order.offsets.numel() - 1)
+
+
+def _scatter(x, order):
+    tokens, topk = order.position.shape
+    out = torch.empty(tokens * topk, x.shape[1], dtype=x.dtype, device=x.device)
+    load().scatter_rows(x.data_ptr(), pitch(x), out.data_ptr(), order.position.data_ptr(), _rows_kept(order), tokens, topk, x.shape[1],
+                        ELEMS[x.dtype], stream_handle())
+    return out
+
+
+def _combine(ys, weights, order):
+    tokens, topk = order.position.shape
+    out = torch.empty(tokens, ys.shape[1], dtype=ys.dtype, device=ys.device)
+    load().combine_rows(ys.data_ptr(), pitch(ys), 0 if weights is None else weights.data_ptr(), out.data_ptr(), order.position.data_ptr(),
+                        _rows_kept(order), tokens, topk, ys.shape[1], ELEMS[ys.dtype], stream_handle())
+    return out
+
+
+def _kernel_rows(g, like):
+    """An incoming gradient as the kernels take it: autograd may hand over an expanded or otherwise strided tensor."""
+    g = g.to(like)
+    unit = 16 // g.element_size()
+    if g.stride(-1) != 1 or g.data_ptr() % 16 or (g.shape[0] > 1 and (g.stride(0) % unit or g.stride(0) <= 0)):
+        g = g.contiguous()
+    return g.clone() if g.data_ptr() % 16 else g
+
+
+class _Gather(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, order):
+        ctx.order, ctx.dtype = order, x.dtype
+        return _scatter(x, order)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dxs):
+        with on_stream(dxs.device, None):
+            return _combine(_kernel_rows(dxs, ctx.dtype), None, ctx.order), None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ys, weights, order):
+        ctx.order = order
+        ctx.save_for_backward(ys, weights)
+        return _combine(ys, weights, order)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        ys, weights = ctx.saved_tensors
+        order = ctx.order
+        tokens, topk = order.position.shape
+        with on_stream(dy.device, None):
+            dy = _kernel_rows(dy, ys.dtype)
+            dys = torch.empty(ys.shape, dtype=ys.dtype, device=ys.device) if ctx.needs_input_grad[0] else None
+            dweights = torch.empty(weights.shape, dtype=weights.dtype, device=ys.device) if ctx.needs_input_grad[1] else None
+            load().combine_backward(dy.data_ptr(), pitch(dy), ys.data_ptr(), pitch(ys), weights.data_ptr(),
+                                    0 if dys is None else dys.data_ptr(), 0 if dweights is None else dweights.data_ptr(),
+                                    order.position.data_ptr(), _rows_kept(order), tokens, topk, ys.shape[1], ELEMS[ys.dtype],
+                                    stream_handle())
+        return dys, dweights, None
+
+
+def gather_rows(x, order, stream=None):
+    """``xs[order.position[t, j]] = x[t]``: the row of every copy, ordered by expert; zeros in the rows of dropped copies.
+    ``x`` [tokens, hidden] fp32, bf16 or fp16, rows of whole 16-byte units.  The gradient of a token is the sum of its copies'
+    (fp32, in the order of ``j``, rounded once)."""
+    _check_rows(x, 'x')
+    tokens = order.position.shape[0]
+    check(x.shape[0] == tokens, f'x has {x.shape[0]} rows, the order {tokens} tokens')
+    with on_stream(check_devices(x=x, order=order.position), stream, x, order.position):
+        return _Gather.apply(x, order) if torch.is_grad_enabled() and x.requires_grad else _scatter(x, order)
+
+
+def combine_rows(ys, weights, order, stream=None):
+    """``y[t] = sum_j weights[t, j] * ys[order.position[t, j]]`` over the copies that were not dropped (those are not even read);
+    fp32 sums in the order of ``j``, rounded once.  ``ys`` [tokens * k, hidden] fp32, bf16 or fp16, ``weights`` [tokens, k] fp32.
+    Gradients: ``ys`` and ``weights`` (zero for dropped copies)."""
+    _check_rows(ys, 'ys')
+    tokens, topk = order.position.shape
+    check(ys.shape[0] == tokens * topk, f'ys has {ys.shape[0]} rows, the order {tokens * topk} copies')
+    check(weights.dtype == torch.float32 and weights.shape == (tokens, topk), f'weights must be a [{tokens}, {topk}] float32 tensor')
+    with on_stream(check_devices(ys=ys, weights=weights, order=order.position), stream, ys, weights, order.position):
+        weights = weights.contiguous()
+        needs = torch.is_grad_enabled() and (ys.requires_grad or weights.requires_grad)
+        return _Combine.apply(ys, weights, order) if needs else _combine(ys, weights, order)
