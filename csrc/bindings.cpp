@@ -618,6 +618,28 @@ PYBIND11_MODULE(_msccl_native, m) {
                                                 k, elem, f32_out, reinterpret_cast<int*>(error_words), as_stream(stream)),
              "launch of the grouped weight gradient kernel");
   });
+  // e4m3 with fp32 scales per 128 values of a row (activations) or per 128 x 128 values (weights).
+  m.def("quantize_rows", [](uintptr_t x, long long ldx, uintptr_t q, uintptr_t scales, long long s_row, long long s_block, int rows, int k, int elem,
+                            uintptr_t stream) {
+    check_rt(msccl::sm100::launch_quantize_rows(reinterpret_cast<const void*>(x), ldx, reinterpret_cast<void*>(q), reinterpret_cast<float*>(scales),
+                                                s_row, s_block, rows, k, elem, as_stream(stream)),
+             "launch of the row quantisation kernel");
+  });
+  m.def("quantize_blocks", [](uintptr_t w, long long ldw, long long lde, uintptr_t q, uintptr_t scales, int groups, int n, int k, int elem,
+                              uintptr_t stream) {
+    check_rt(msccl::sm100::launch_quantize_blocks(reinterpret_cast<const void*>(w), ldw, lde, reinterpret_cast<void*>(q),
+                                                  reinterpret_cast<float*>(scales), groups, n, k, elem, as_stream(stream)),
+             "launch of the block quantisation kernel");
+  });
+  m.def("fp8_block_gemm", [](uintptr_t a, long long lda, uintptr_t sa, long long sa_row, long long sa_block, uintptr_t w, long long ldw, long long lde,
+                             uintptr_t sb, uintptr_t offsets, uintptr_t out, long long ldo, int rows, int groups, int n, int k, int bn,
+                             bool few_rows, bool zero_rest, uintptr_t error_words, uintptr_t stream) {
+    check_rt(msccl::sm100::launch_fp8_block_gemm(reinterpret_cast<const void*>(a), lda, reinterpret_cast<const float*>(sa), sa_row, sa_block,
+                                                 reinterpret_cast<const void*>(w), ldw, lde, reinterpret_cast<const float*>(sb),
+                                                 reinterpret_cast<const int*>(offsets), reinterpret_cast<void*>(out), ldo, rows, groups, n, k, bn,
+                                                 few_rows, zero_rest, reinterpret_cast<int*>(error_words), as_stream(stream)),
+             "launch of the block-scaled fp8 GEMM kernel");
+  });
   // Gradient norm and clipping of a list of tensors (grad_norm.cu).
   py::class_<GradList>(m, "GradList")
       .def(py::init<const py::list&, const py::object&, const py::tuple&, const py::function&>())

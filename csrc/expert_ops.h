@@ -1,5 +1,5 @@
 // Host API of the operators of an expert layer: row exchange (moe_rows.cu), grouped products
-// (grouped_gemm.cu, grouped_wgrad.cu), gradient norm (grad_norm.cu).
+// (grouped_gemm.cu, grouped_wgrad.cu), block-scaled fp8 (fp8_block_gemm.cu, quantize_block.cu), gradient norm (grad_norm.cu).
 #pragma once
 #include <cuda_runtime.h>
 
@@ -30,6 +30,15 @@ cudaError_t launch_grouped_gemm(const void* x, long long ldx, const void* w, lon
 cudaError_t launch_grouped_wgrad(const void* dy, long long lddy, const void* x, long long ldx, const int* offsets, void* out, long long ldo,
                                  long long lde, int rows, int groups, int n, int k, int elem, bool f32_out, int* error_words,
                                  cudaStream_t stream);
+
+// ---- 8-bit floating point with fp32 scales per block of 128 (fp8_block_gemm.cu, quantize_block.cu)
+cudaError_t launch_quantize_rows(const void* x, long long ldx, void* q, float* scales, long long s_row, long long s_block, int rows, int k,
+                                 int elem, cudaStream_t stream);
+cudaError_t launch_quantize_blocks(const void* w, long long ldw, long long lde, void* q, float* scales, int groups, int n, int k, int elem,
+                                   cudaStream_t stream);
+cudaError_t launch_fp8_block_gemm(const void* a, long long lda, const float* sa, long long sa_row, long long sa_block, const void* w,
+                                  long long ldw, long long lde, const float* sb, const int* offsets, void* out, long long ldo, int rows,
+                                  int groups, int n, int k, int bn, bool few_rows, bool zero_rest, int* error_words, cudaStream_t stream);
 
 // ---- gradient norm and clipping
 struct GradTensor {

@@ -1,0 +1,338 @@
+// Products in 8-bit floating point with fp32 scales per block of 128, for sm_100a, dense or by group:
+//
+//   d[t, n] = sum over blocks b of K:  sa[t, b] * sb[e, n / 128, b] * (sum over k in b of a[t, k] w[e, n, k])
+//
+// a, w: e4m3; sa: one scale per row and 128 values; sb: one per 128 x 128 values; d: bf16.
+//
+// The scales are arbitrary fp32 numbers, so the tensor core cannot apply them (its block scales are powers of two): every block of
+// K gets an accumulator of its own in tensor memory (tcgen05.mma kind::f8f6f4, four instructions of K = 32), and eight warps add
+// scale * accumulator to fp32 sums in registers while the tensor core fills the next accumulator.  The lane of an accumulator is
+// a row, so that one number per thread and block scales all of its columns.  Tiles are 128 rows x BN columns of one CTA: warps
+// 2 .. 9 take a quarter of the rows and half of the columns each.
+//
+// With at most 32 rows in every tile only 32 rows of `a` are loaded; the tensor core then reads whatever follows in shared memory
+// as the other rows (still inside the allocation) and their results are not read.
+//
+// Every wait is bounded (gemm_sm100.cuh).
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "expert_ops.h"
+#include "gemm_sm100.cuh"
+#include "gemm_sm100.h"
+#include "grouped_common.cuh"
+
+namespace msccl {
+namespace sm100 {
+
+namespace {
+
+constexpr int kFThreads = 320;                   // 0 producer, 1 MMA, 2..9 scaling and epilogue
+constexpr int kFEpilogueWarps = 8;
+constexpr int kFBlock = 128;                     // K values per scale = bytes per shared-memory row
+constexpr int kFGroupTileRows = 2048;
+constexpr int kFSmemLimit = 216 * 1024;
+
+template <int BN, int AR> struct FGeometry {
+  static constexpr int kABytes = AR * kFBlock;
+  static constexpr int kBBytes = BN * kFBlock;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kBehind = (BM - AR) * kFBlock;       // what the MMA reads behind the rows of the last stage
+  static constexpr int kFit = (kFSmemLimit - kBehind) / kStageBytes;
+  static constexpr int kStages = kFit < 16 ? kFit : 16;
+  static constexpr int kAccs = 512 / BN < 4 ? 512 / BN : 4;
+  static constexpr int kTmemCols = kAccs * BN;
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStageBytes + kBehind + 512;
+};
+
+struct FArgs {
+  const int* offsets;                            // nullptr: one group of all rows
+  const float *sa, *sb;
+  long long sa_row, sa_block;                    // strides of sa
+  __nv_bfloat16* out;
+  long long ldo;
+  int rows, groups, n, k;
+  int zero_rest;
+  int* error_words;
+};
+
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// Two fp32 sums at once: acc += scale * v.
+__device__ __forceinline__ void fma2(float2& acc, float2 scale, uint32_t lo, uint32_t hi) {
+  unsigned long long a, s, v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(acc.x), "f"(acc.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(s) : "f"(scale.x), "f"(scale.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(s), "l"(v));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(acc.x), "=f"(acc.y) : "l"(a));
+}
+
+template <int BN, int AR>
+__global__ void __launch_bounds__(kFThreads, 1)
+fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const FArgs g) {
+  using Geo = FGeometry<BN, AR>;
+  constexpr int S = Geo::kStages, ACCS = Geo::kAccs;
+  constexpr int COLS = BN / 2;                   // columns of one epilogue thread
+  constexpr int CHUNK = COLS < 32 ? COLS : 32;
+  static_assert(CHUNK == 32 || CHUNK == 16, "");
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ GroupTable table;
+  uint8_t* stage_base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stage_base + static_cast<size_t>(S) * Geo::kStageBytes + Geo::kBehind);
+  uint64_t *full_bar = bars, *empty_bar = bars + S, *acc_full = bars + 2 * S, *acc_empty = bars + 2 * S + ACCS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 2 * ACCS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int n_tiles = (g.n + BN - 1) / BN;
+  const int k_blocks = (g.k + kFBlock - 1) / kFBlock;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < ACCS; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], kFEpilogueWarps);
+    }
+    // an earlier launch gave up: every role leaves at its first wait
+    *abort_flag = g.error_words != nullptr && *reinterpret_cast<volatile int*>(g.error_words) != 0 ? 1 : 0;
+    mbar_fence_init();
+    prefetch_tensormap(&map_a);
+    prefetch_tensormap(&map_w);
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, Geo::kTmemCols);
+  if (warp == 2) {
+    auto tiles_of = [&](int rows) { return (rows + BM - 1) / BM * n_tiles; };
+    if (g.offsets != nullptr) {
+      build_groups(table, g.offsets, g.groups, g.rows, tiles_of);
+    } else if (lane == 0) {
+      table.row_start[0] = table.tile_start[0] = 0;
+      table.row_start[1] = g.rows;
+      table.tile_start[1] = tiles_of(g.rows);
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  const bool skip = *abort_flag != 0;
+  const int num_tiles = skip ? 0 : table.tile_start[g.groups];
+  __syncthreads();                               // nobody raises the flag before everybody has read it
+
+  auto locate = [&](int tile, int& e, int& row, int& column) {
+    while (tile >= table.tile_start[e + 1]) ++e;
+    const int rows = table.row_start[e + 1] - table.row_start[e];
+    int tm, tn;
+    tile_coords(tile - table.tile_start[e], (rows + BM - 1) / BM, n_tiles, kFGroupTileRows / BM, tm, tn);
+    row = table.row_start[e] + tm * BM;
+    column = tn * BN;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0, e = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+        int row, column;
+        locate(tile, e, row, column);
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) {
+            gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_EMPTY, 0, stage);
+            ok = false;
+            break;
+          }
+          uint8_t* a_dst = stage_base + static_cast<size_t>(stage) * Geo::kStageBytes;
+          mbar_expect_tx(&full_bar[stage], Geo::kStageBytes);
+          tma_load_2d(a_dst, &map_a, &full_bar[stage], kb * kFBlock, row);
+          tma_load_3d(a_dst + Geo::kABytes, &map_w, &full_bar[stage], kb * kFBlock, column, e);
+          if (++stage == S) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok) drain_wait();
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>(BM >> 4) << 24);   // e4m3 x e4m3 -> fp32
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1, abort_flag)) {
+            gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 1, acc);
+            ok = false;
+            break;
+          }
+          if (!mbar_wait(&full_bar[stage], phase, abort_flag)) {
+            gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_FULL, 1, stage);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t a_addr = smem_u32(stage_base + static_cast<size_t>(stage) * Geo::kStageBytes);
+          const uint64_t adesc = smem_desc_sw128(a_addr), bdesc = smem_desc_sw128(a_addr + Geo::kABytes);
+          const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * BN);
+#pragma unroll
+          for (int k = 0; k < kFBlock / 32; ++k)
+            umma_f8(tmem_d, adesc + static_cast<uint64_t>(k * 2), bdesc + static_cast<uint64_t>(k * 2), idesc, k != 0);
+          tc_commit(&empty_bar[stage]);
+          tc_commit(&acc_full[acc]);
+          if (++stage == S) { stage = 0; phase ^= 1; }
+          if (++acc == ACCS) { acc = 0; acc_phase ^= 1; }
+        }
+      }
+    }
+  } else {
+    const int quarter = warp % 4, half = (warp - 2) / 4;
+    int acc = 0, e = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      int row, column;
+      locate(tile, e, row, column);
+      const int left = table.row_start[e + 1] - row - quarter * 32;       // rows of this warp that are the group's
+      row += quarter * 32 + lane;
+      column += half * COLS;
+      const float* sa = g.sa + min(row, g.rows - 1) * g.sa_row;
+      const int sb_rows = (g.n + kFBlock - 1) / kFBlock;
+      const float* sb = g.sb + (static_cast<long long>(e) * sb_rows + min(column / kFBlock, sb_rows - 1)) * k_blocks;
+      float2 sum[COLS / 2];
+#pragma unroll
+      for (int i = 0; i < COLS / 2; ++i) sum[i] = make_float2(0.0f, 0.0f);
+      float next = left > 0 ? sa[0] * sb[0] : 0.0f;
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        const float scale = next;
+        if (left > 0 && kb + 1 < k_blocks) next = sa[(kb + 1) * g.sa_block] * sb[kb + 1];
+        ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag);
+        ok = __all_sync(kFullMask, ok);
+        if (!ok) {
+          if (lane == 0) gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 2, acc);
+          break;
+        }
+        tc_fence_after_sync();
+        if (left > 0) {
+          const float2 s2 = make_float2(scale, scale);
+          const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BN + half * COLS);
+#pragma unroll
+          for (int c = 0; c < COLS; c += CHUNK) {
+            if constexpr (CHUNK == 32) {
+              uint32_t r[32];
+              tmem_ld32(taddr + c, r);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) fma2(sum[c / 2 + i], s2, r[2 * i], r[2 * i + 1]);
+            } else {
+              uint32_t r[16];
+              tmem_ld16(taddr + c, r);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 8; ++i) fma2(sum[c / 2 + i], s2, r[2 * i], r[2 * i + 1]);
+            }
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[acc]);
+        if (++acc == ACCS) { acc = 0; acc_phase ^= 1; }
+      }
+      if (ok && lane < left) {
+        __nv_bfloat16* out = g.out + row * g.ldo + column;
+#pragma unroll
+        for (int c = 0; c < COLS; c += 8)
+          if (column + c < g.n)
+            *reinterpret_cast<uint4*>(out + c) = make_uint4(pack_bf16(sum[c / 2].x, sum[c / 2].y), pack_bf16(sum[c / 2 + 1].x, sum[c / 2 + 1].y),
+                                                            pack_bf16(sum[c / 2 + 2].x, sum[c / 2 + 2].y), pack_bf16(sum[c / 2 + 3].x, sum[c / 2 + 3].y));
+      }
+    }
+    if (g.zero_rest && !skip) {
+      const int head = table.row_start[0], tail = table.row_start[g.groups];
+      const int rest = head + g.rows - tail;
+      for (int i = blockIdx.x * kFEpilogueWarps + warp - 2; i < rest; i += gridDim.x * kFEpilogueWarps) {
+        uint4* dst = reinterpret_cast<uint4*>(g.out + static_cast<long long>(i < head ? i : tail + i - head) * g.ldo);
+        for (int v = lane; v < g.n / 8; v += 32) dst[v] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, Geo::kTmemCols);
+  }
+}
+
+template <int BN, int AR>
+cudaError_t launch(const CUtensorMap& map_a, const CUtensorMap& map_w, const FArgs& g, int most_tiles, cudaStream_t stream) {
+  auto kernel = fp8_block_kernel<BN, AR>;
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(FGeometry<BN, AR>::kSmem));
+  if (err != cudaSuccess) return err;
+  kernel<<<most_tiles < sm_count() ? most_tiles : sm_count(), kFThreads, FGeometry<BN, AR>::kSmem, stream>>>(map_a, map_w, g);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+// a: [rows, k] e4m3 (pitch lda bytes), sa: [rows, ceil(k / 128)] with the strides given; w: [groups, n, k] e4m3 (pitch ldw, matrix
+// stride lde), sb: [groups, ceil(n / 128), ceil(k / 128)] contiguous; out: [rows, n] bf16.  k % 16 == 0, n % 8 == 0.
+// bn: 32, 64, 128 or 256; few_rows: no group has more than 32 rows.
+cudaError_t launch_fp8_block_gemm(const void* a, long long lda, const float* sa, long long sa_row, long long sa_block, const void* w,
+                                  long long ldw, long long lde, const float* sb, const int* offsets, void* out, long long ldo, int rows,
+                                  int groups, int n, int k, int bn, bool few_rows, bool zero_rest, int* error_words, cudaStream_t stream) {
+  if (rows < 1 || groups < 1 || groups > kMaxGroups || n < 8 || k < 16 || n % 8 != 0 || k % 16 != 0 || lda % 16 != 0 || ldw % 16 != 0 ||
+      lde % 16 != 0 || ldo % 8 != 0 || (offsets == nullptr && groups != 1) || (few_rows && rows > 32))
+    return cudaErrorInvalidValue;
+  FArgs g;
+  g.offsets = offsets;
+  g.sa = sa;
+  g.sb = sb;
+  g.sa_row = sa_row;
+  g.sa_block = sa_block;
+  g.out = static_cast<__nv_bfloat16*>(out);
+  g.ldo = ldo;
+  g.rows = rows;
+  g.groups = groups;
+  g.n = n;
+  g.k = k;
+  g.zero_rest = zero_rest ? 1 : 0;
+  g.error_words = error_words;
+  const uint64_t a_dims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(rows)}, a_strides[1] = {static_cast<uint64_t>(lda)};
+  const uint32_t a_box[2] = {kFBlock, few_rows ? 32u : static_cast<uint32_t>(BM)};
+  const CUtensorMap map_a = make_swizzled_map(a, 1, 2, a_dims, a_strides, a_box);
+  const uint64_t w_dims[3] = {static_cast<uint64_t>(k), static_cast<uint64_t>(n), static_cast<uint64_t>(groups)};
+  const uint64_t w_strides[2] = {static_cast<uint64_t>(ldw), static_cast<uint64_t>(lde)};
+  const uint32_t w_box[3] = {kFBlock, static_cast<uint32_t>(bn), 1};
+  const CUtensorMap map_w = make_swizzled_map(w, 1, 3, w_dims, w_strides, w_box);
+  const long long active = groups < rows ? groups : rows, most = static_cast<long long>((n + bn - 1) / bn) * (rows / BM + active);
+  if (most > (1ll << 30)) return cudaErrorInvalidValue;
+  const int tiles = static_cast<int>(most);
+  switch (bn) {
+    case 32: return few_rows ? launch<32, 32>(map_a, map_w, g, tiles, stream) : launch<32, BM>(map_a, map_w, g, tiles, stream);
+    case 64: return few_rows ? launch<64, 32>(map_a, map_w, g, tiles, stream) : launch<64, BM>(map_a, map_w, g, tiles, stream);
+    case 128: return few_rows ? launch<128, 32>(map_a, map_w, g, tiles, stream) : launch<128, BM>(map_a, map_w, g, tiles, stream);
+    case 256: return few_rows ? launch<256, 32>(map_a, map_w, g, tiles, stream) : launch<256, BM>(map_a, map_w, g, tiles, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace sm100
+}  // namespace msccl

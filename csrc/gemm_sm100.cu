@@ -228,6 +228,14 @@ EncodeTiledFn encode_fn() {
       throw std::runtime_error("cuTensorMapEncodeTiled is not available");
     fn = reinterpret_cast<EncodeTiledFn>(p);
   }
+  // A driver call needs a context on its thread.  A thread that has made no runtime call yet (autograd runs the backward pass on
+  // one of its own) has none until it sets its device.
+  thread_local bool bound = false;
+  if (!bound) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) throw std::runtime_error("no CUDA device is current");
+    bound = true;
+  }
   return fn;
 }
 

@@ -1,0 +1,125 @@
+"""Products in 8-bit floating point (e4m3) with fp32 scales: one per 128 values of an activation row, one per 128 x 128 values of a
+weight (``csrc/fp8_block_gemm.cu``, ``csrc/quantize_block.cu``).  Weights are quantised once, activations per call:
+
+    wq, ws = quantize_fp8_block_weight(w)                 # w [n, k], or [experts, n, k]
+    xq, xs = quantize_fp8_block(x)                        # x [rows, k]
+    y = gemm_fp8_block(xq, xs, wq, ws)                    # bf16 [rows, n]
+    y = grouped_gemm_fp8_block(xq, xs, wq, ws, offsets)   # rows of expert e: offsets[e] .. offsets[e + 1]
+
+Beside the MX format of ``msccl.ops.gemm`` (a power of two per 32 values, applied inside the tensor core) these scales are any
+fp32 numbers, the form in which block-quantised checkpoints come.  There are no gradients: this is the path for serving.
+"""
+import torch
+
+from msccl.ops._launch import (ELEMS, check, check_apart, check_devices, check_matrix, check_offsets, error_words, on_stream, pitch,
+                               stream_handle)
+from msccl.ops.moe_rows import MAX_EXPERTS
+from msccl.runtime.native import load
+
+BLOCK = 128
+_E4M3 = torch.float8_e4m3fn
+
+
+def _blocks(size):
+    return -(-size // BLOCK)
+
+
+def quantize_fp8_block(x, stream=None):
+    """``x`` [rows, k] fp32, bf16 or fp16 (k a multiple of 16) -> ``(q, scales)``: e4m3 [rows, k] and float32 [rows, ceil(k / 128)].
+    ``scale = max(largest magnitude, 2 ** -100) / 448`` over the block, ``q = e4m3(x / scale)``, each rounded once.  The scales
+    of neighbouring rows lie next to each other in memory, as the product reads them.  A NaN or an infinity makes its block NaN
+    (or zero beside an infinity)."""
+    check_matrix(x, 'x', ELEMS, 16)
+    device = check_devices(x=x)
+    with on_stream(device, stream, x):
+        rows, k = x.shape
+        q = torch.empty(rows, k, dtype=_E4M3, device=device)
+        scales = torch.empty(_blocks(k), rows, dtype=torch.float32, device=device).t()
+        if rows:
+            load().quantize_rows(x.data_ptr(), pitch(x), q.data_ptr(), scales.data_ptr(), 1, rows, rows, k, ELEMS[x.dtype], stream_handle())
+    return q, scales
+
+
+def quantize_fp8_block_weight(w, stream=None):
+    """``w`` [n, k] or [experts, n, k] -> e4m3 of the same shape and float32 scales [.., ceil(n / 128), ceil(k / 128)], by the rule of
+    ``quantize_fp8_block`` over blocks of 128 x 128."""
+    check(w.dim() in (2, 3), f'w must be [n, k] or [experts, n, k] (got {w.dim()} dimensions)')
+    check_matrix(w, 'w', ELEMS, 16, dims=w.dim())
+    check(w.numel() > 0, 'w is empty')
+    device = check_devices(w=w)
+    n, k = w.shape[-2:]
+    experts = w.shape[0] if w.dim() == 3 else 1
+    check(experts <= 65535, f'at most 65535 matrices at once (got {experts})')
+    with on_stream(device, stream, w):
+        q = torch.empty(w.shape, dtype=_E4M3, device=device)
+        scales = torch.empty(*w.shape[:-2], _blocks(n), _blocks(k), dtype=torch.float32, device=device)
+        load().quantize_blocks(w.data_ptr(), pitch(w), w.stride(0) if experts > 1 else n * pitch(w), q.data_ptr(), scales.data_ptr(), experts, n,
+                               k, ELEMS[w.dtype], stream_handle())
+    return q, scales
+
+
+def dequantize_fp8_block(q, scales):
+    """fp32 values of a ``quantize_fp8_block`` or ``quantize_fp8_block_weight`` pair (on any device)."""
+    s = scales.repeat_interleave(BLOCK, -1)[..., :q.shape[-1]]
+    if scales.shape[-2] != q.shape[-2]:
+        s = s.repeat_interleave(BLOCK, -2)[..., :q.shape[-2], :]
+    return q.float() * s
+
+
+def _tile_columns(rows, groups, n):
+    """Columns per tile: see csrc/fp8_block_gemm.cu."""
+    row_tiles = rows // 128 + min(rows, groups)
+    for bn in (256, 128, 64):
+        if row_tiles * -(-n // bn) >= 148:
+            return bn
+    return 32
+
+
+def _check(a, sa, w, sw, offsets, out, dims):
+    check_matrix(w, 'w', (_E4M3,), 16, dims=dims)
+    n, k = w.shape[-2:]
+    check(n > 0 and n % 8 == 0, f'the rows of a weight must be a positive multiple of 8 (got {n})')
+    check_matrix(a, 'a', (_E4M3,), 16)
+    check(a.shape[1] == k, f'inner dimensions differ (a {a.shape[1]}, w {k})')
+    check(sa.dtype == torch.float32 and sa.shape == (a.shape[0], _blocks(k)) and all(s >= 0 for s in sa.stride()),
+          f'the scales of a must be float32 [{a.shape[0]}, {_blocks(k)}] (got {sa.dtype} {list(sa.shape)})')
+    want = (*w.shape[:-2], _blocks(n), _blocks(k))
+    check(sw.dtype == torch.float32 and sw.shape == want and sw.is_contiguous(),
+          f'the scales of w must be contiguous float32 {list(want)} (got {sw.dtype} {list(sw.shape)})')
+    if offsets is not None:
+        check(1 <= w.shape[0] <= MAX_EXPERTS, f'between 1 and {MAX_EXPERTS} experts are supported (got {w.shape[0]})')
+        check_offsets(offsets, w.shape[0])
+    if out is not None:
+        check_matrix(out, 'out', (torch.bfloat16,), 8)
+        check(out.shape == (a.shape[0], n), f'out must be [{a.shape[0]}, {n}] (got {list(out.shape)})')
+        check_apart(out, a=a, sa=sa, w=w, sw=sw)
+    return check_devices(a=a, sa=sa, w=w, sw=sw, offsets=offsets, out=out)
+
+
+def _product(a, sa, w, sw, offsets, out, stream, dims):
+    device = _check(a, sa, w, sw, offsets, out, dims)
+    with on_stream(device, stream, *(t for t in (a, sa, w, sw, offsets, out) if t is not None)):
+        rows, (n, k) = a.shape[0], w.shape[-2:]
+        groups = w.shape[0] if dims == 3 else 1
+        zero_rest = out is None and offsets is not None
+        if out is None:
+            out = torch.empty(rows, n, dtype=torch.bfloat16, device=device)
+        if rows:
+            load().fp8_block_gemm(a.data_ptr(), pitch(a), sa.data_ptr(), sa.stride(0), sa.stride(1), w.data_ptr(), pitch(w),
+                                  w.stride(0) if groups > 1 else n * pitch(w), sw.data_ptr(), 0 if offsets is None else offsets.data_ptr(),
+                                  out.data_ptr(), pitch(out), rows, groups, n, k, _tile_columns(rows, groups, n), rows <= 32, zero_rest,
+                                  error_words(device), stream_handle())
+    return out
+
+
+def gemm_fp8_block(a, sa, w, sw, out=None, stream=None):
+    """bf16 [rows, n] = dequant(a) @ dequant(w).T, sums in fp32.  ``a`` [rows, k] with ``sa`` [rows, ceil(k / 128)] (any strides) from
+    ``quantize_fp8_block``; ``w`` [n, k] with ``sw`` from ``quantize_fp8_block_weight``; k a multiple of 16, n of 8."""
+    return _product(a, sa, w, sw, None, out, stream, 2)
+
+
+def grouped_gemm_fp8_block(a, sa, w, sw, offsets, out=None, stream=None):
+    """The same with a weight for each expert: rows ``offsets[e] .. offsets[e + 1]`` times ``w[e]``.  ``offsets`` and rows of no expert
+    as in ``msccl.ops.grouped``."""
+    check(offsets is not None, 'offsets are needed')
+    return _product(a, sa, w, sw, offsets, out, stream, 3)

@@ -216,6 +216,41 @@ def test_captured_and_on_another_stream():
             assert torch.equal(dw, _weight_gradient(dy, x, at).bfloat16())
 
 
+@pytest.mark.parametrize('what', ['forward', 'backward'])
+def test_first_call_of_a_thread(what):
+    """A thread that has made no CUDA call yet, as autograd's are at first (in a process of its own: contexts outlive a test)."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys, threading, torch
+from msccl.ops import check_gemm_errors
+from msccl.ops.grouped import grouped_gemm
+x = torch.randn(64, 64, device='cuda').bfloat16()
+w = torch.randn(2, 64, 64, device='cuda').bfloat16()
+offsets = torch.tensor([0, 30, 64], dtype=torch.int32, device='cuda')
+failed = []
+def call():
+    try:
+        grouped_gemm(x, w, offsets)
+    except Exception as e:
+        failed.append(e)
+if sys.argv[1] == 'forward':
+    t = threading.Thread(target=call)
+    t.start()
+    t.join()
+else:
+    x.requires_grad_()
+    y = grouped_gemm(x, w, offsets)
+    torch.autograd.grad(y, x, torch.ones_like(y))
+check_gemm_errors()
+assert not failed, failed
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, '-c', code, what], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stdout + done.stderr
+
+
 def test_far_rows():
     """Offsets of elements beyond 2^31: 150000 rows of 16384 columns."""
     from msccl.ops import check_gemm_errors
