@@ -284,8 +284,16 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 template <int BN, int AR>
 cudaError_t launch(const CUtensorMap& map_a, const CUtensorMap& map_w, const FArgs& g, int most_tiles, cudaStream_t stream) {
   auto kernel = fp8_block_kernel<BN, AR>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(FGeometry<BN, AR>::kSmem));
+  static bool ready[64] = {};
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!ready[dev]) {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(FGeometry<BN, AR>::kSmem));
+    if (err != cudaSuccess) return err;
+    ready[dev] = true;
+  }
   kernel<<<most_tiles < sm_count() ? most_tiles : sm_count(), kFThreads, FGeometry<BN, AR>::kSmem, stream>>>(map_a, map_w, g);
   return cudaGetLastError();
 }

@@ -1,4 +1,8 @@
-"""What the expert-layer operators share: element types, argument checks, and the device and stream of a call."""
+"""What the expert-layer operators share: element types, argument checks, and the device and stream of a call.
+
+A call on a few tokens takes a handful of microseconds on the GPU, so the checks of a valid call are a few comparisons each;
+messages are only put together once one has failed.
+"""
 import contextlib
 
 import torch
@@ -7,8 +11,8 @@ ELEMS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # ElemTyp
 
 
 @contextlib.contextmanager
-def _elsewhere(device, stream):
-    with torch.cuda.device(device):
+def _elsewhere(index, stream):
+    with torch.cuda.device(index):
         if stream is None:
             yield
         else:
@@ -17,22 +21,27 @@ def _elsewhere(device, stream):
 
 
 _HERE = contextlib.nullcontext()
+# the public torch.cuda.current_device() and current_stream().cuda_stream give the same numbers in five microseconds more
+_current_device = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.current_device
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def on_stream(device, stream, *tensors):
-    """Context in which a call on tensors of ``device`` allocates and launches: that device is current and, with ``stream``,
-    that stream too.  ``tensors`` then stay allocated until the work on ``stream`` that was queued meanwhile is done."""
+def on_stream(index, stream, tensors=()):
+    """Context in which a call on tensors of device ``index`` allocates and launches: that device is current and, with ``stream``,
+    that stream too.  ``tensors`` (``None`` ones apart) then stay allocated until the work on ``stream`` that was queued
+    meanwhile is done."""
     if stream is None:
-        return _HERE if torch.cuda.current_device() == device.index else _elsewhere(device, None)
-    if stream.device != device:
-        raise ValueError(f'the stream belongs to {stream.device}, the tensors to {device}')
+        return _HERE if _current_device() == index else _elsewhere(index, None)
+    if stream.device.index != index:
+        raise ValueError(f'the stream belongs to {stream.device}, the tensors to cuda:{index}')
     for t in tensors:
-        t.record_stream(stream)
-    return _elsewhere(device, stream)
+        if t is not None:
+            t.record_stream(stream)
+    return _elsewhere(index, stream)
 
 
-def stream_handle():
-    return torch.cuda.current_stream().cuda_stream
+def stream_handle(index):
+    return _raw_stream(index)
 
 
 def check(condition, message):
@@ -43,34 +52,44 @@ def check(condition, message):
 def check_matrix(t, name, dtypes, unit, dims=2):
     """``t`` has ``dims`` dimensions, its rows are contiguous, start on 16-byte boundaries and hold a multiple of ``unit`` elements.
     A stride that no index uses (one row, one matrix) may have any value."""
-    check(t.dtype in dtypes, f'{name} must be {" or ".join(str(d) for d in dtypes)} (got {t.dtype})')
-    check(t.dim() == dims, f'{name} must have {dims} dimensions (got {t.dim()})')
-    check(t.shape[-1] > 0 and t.shape[-1] % unit == 0, f'the last dimension of {name} must be a positive multiple of {unit} (got {t.shape[-1]})')
-    check(t.stride(-1) == 1, f'the rows of {name} must be contiguous')
-    step = 16 // t.element_size()
-    inner = t.shape[-1]
+    shape, stride, dtype = t.shape, t.stride(), t.dtype
+    if dtype not in dtypes:
+        raise ValueError(f'{name} must be {" or ".join(str(d) for d in dtypes)} (got {dtype})')
+    if len(shape) != dims:
+        raise ValueError(f'{name} must have {dims} dimensions (got {len(shape)})')
+    inner = shape[-1]
+    if inner <= 0 or inner % unit:
+        raise ValueError(f'the last dimension of {name} must be a positive multiple of {unit} (got {inner})')
+    if stride[-1] != 1:
+        raise ValueError(f'the rows of {name} must be contiguous')
+    step = 16 // dtype.itemsize
     for d in range(dims - 2, -1, -1):
-        check(t.shape[d] <= 1 or t.stride(d) % step == 0 and t.stride(d) >= inner,
-              f'the strides of {name} must be multiples of 16 bytes and its rows must not overlap (stride {t.stride(d)})')
-        inner = max(inner, t.stride(d) * t.shape[d] if t.shape[d] > 1 else inner)
-    check(t.data_ptr() % 16 == 0, f'{name} must start on a 16-byte boundary')
+        if shape[d] > 1:
+            if stride[d] % step or stride[d] < inner:
+                raise ValueError(f'the strides of {name} must be multiples of 16 bytes and its rows must not overlap (stride {stride[d]})')
+            inner = stride[d] * shape[d]
+    if t.data_ptr() % 16:
+        raise ValueError(f'{name} must start on a 16-byte boundary')
 
 
 def check_offsets(offsets, experts):
-    check(offsets.dtype == torch.int32 and offsets.shape == (experts + 1,) and offsets.is_contiguous(),
-          f'offsets must be a contiguous [{experts + 1}] int32 tensor (got {list(offsets.shape)} {offsets.dtype})')
+    if offsets.dtype != torch.int32 or offsets.shape != (experts + 1,) or offsets.stride(0) != 1:
+        raise ValueError(f'offsets must be a contiguous [{experts + 1}] int32 tensor (got {list(offsets.shape)} {offsets.dtype})')
 
 
 def check_devices(**tensors):
-    """All tensors (``None`` ones apart) are on one CUDA device; returns it."""
-    device = None
+    """All tensors (``None`` ones apart) are on one CUDA device; returns its index."""
+    index = None
     for name, t in tensors.items():
-        if t is None:
-            continue
-        check(t.is_cuda, f'{name} must be a CUDA tensor')
-        check(device is None or t.device == device, f'{name} is on {t.device}, the other tensors on {device}')
-        device = t.device
-    return device
+        if t is not None:
+            at = t.get_device()
+            if at != index:
+                if at < 0 or not t.is_cuda:
+                    raise ValueError(f'{name} must be a CUDA tensor')
+                if index is not None:
+                    raise ValueError(f'{name} is on cuda:{at}, the other tensors on cuda:{index}')
+                index = at
+    return index
 
 
 def check_apart(out, **inputs):
@@ -78,7 +97,8 @@ def check_apart(out, **inputs):
     lo, hi = span(out)
     for name, t in inputs.items():
         a, b = span(t)
-        check(b <= lo or hi <= a, f'out overlaps {name}')
+        if lo < b and a < hi:
+            raise ValueError(f'out overlaps {name}')
 
 
 def span(t):
@@ -93,9 +113,20 @@ def pitch(t):
     return t.stride(-2) if t.shape[-2] > 1 else t.shape[-1]
 
 
-def error_words(device):
-    """The words in which the GEMM kernels of ``device`` report a wait that ran out (``check_gemm_errors``)."""
-    from msccl.ops import gemm
-    if device.index not in gemm._error_words and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError('call a GEMM of this package once on the device before capturing one into a graph')
-    return gemm._errors(device).data_ptr()
+def matrix_stride(t):
+    """Distance between the matrices of a [count, n, k] tensor in elements."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * pitch(t)
+
+
+_words = {}
+
+
+def error_words(index):
+    """Address of the words in which the GEMM kernels of device ``index`` report a wait that ran out (``check_gemm_errors``)."""
+    address = _words.get(index)
+    if address is None:
+        from msccl.ops.gemm import _error_words, _errors
+        if index not in _error_words and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('call a GEMM of this package once on the device before capturing one into a graph')
+        address = _words[index] = _errors(torch.device('cuda', index)).data_ptr()
+    return address

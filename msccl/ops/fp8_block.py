@@ -11,8 +11,8 @@ fp32 numbers, the form in which block-quantised checkpoints come.  There are no 
 """
 import torch
 
-from msccl.ops._launch import (ELEMS, check, check_apart, check_devices, check_matrix, check_offsets, error_words, on_stream, pitch,
-                               stream_handle)
+from msccl.ops._launch import (ELEMS, check, check_apart, check_devices, check_matrix, check_offsets, error_words, matrix_stride, on_stream,
+                               pitch, stream_handle)
 from msccl.ops.moe_rows import MAX_EXPERTS
 from msccl.runtime.native import load
 
@@ -30,13 +30,13 @@ def quantize_fp8_block(x, stream=None):
     of neighbouring rows lie next to each other in memory, as the product reads them.  A NaN or an infinity makes its block NaN
     (or zero beside an infinity)."""
     check_matrix(x, 'x', ELEMS, 16)
-    device = check_devices(x=x)
-    with on_stream(device, stream, x):
+    index = check_devices(x=x)
+    with on_stream(index, stream, (x,)):
         rows, k = x.shape
-        q = torch.empty(rows, k, dtype=_E4M3, device=device)
-        scales = torch.empty(_blocks(k), rows, dtype=torch.float32, device=device).t()
+        q = torch.empty(rows, k, dtype=_E4M3, device=x.device)
+        scales = torch.empty(_blocks(k), rows, dtype=torch.float32, device=x.device).t()
         if rows:
-            load().quantize_rows(x.data_ptr(), pitch(x), q.data_ptr(), scales.data_ptr(), 1, rows, rows, k, ELEMS[x.dtype], stream_handle())
+            load().quantize_rows(x.data_ptr(), pitch(x), q.data_ptr(), scales.data_ptr(), 1, rows, rows, k, ELEMS[x.dtype], stream_handle(index))
     return q, scales
 
 
@@ -46,15 +46,15 @@ def quantize_fp8_block_weight(w, stream=None):
     check(w.dim() in (2, 3), f'w must be [n, k] or [experts, n, k] (got {w.dim()} dimensions)')
     check_matrix(w, 'w', ELEMS, 16, dims=w.dim())
     check(w.numel() > 0, 'w is empty')
-    device = check_devices(w=w)
+    index = check_devices(w=w)
     n, k = w.shape[-2:]
     experts = w.shape[0] if w.dim() == 3 else 1
     check(experts <= 65535, f'at most 65535 matrices at once (got {experts})')
-    with on_stream(device, stream, w):
-        q = torch.empty(w.shape, dtype=_E4M3, device=device)
-        scales = torch.empty(*w.shape[:-2], _blocks(n), _blocks(k), dtype=torch.float32, device=device)
-        load().quantize_blocks(w.data_ptr(), pitch(w), w.stride(0) if experts > 1 else n * pitch(w), q.data_ptr(), scales.data_ptr(), experts, n,
-                               k, ELEMS[w.dtype], stream_handle())
+    with on_stream(index, stream, (w,)):
+        q = torch.empty(w.shape, dtype=_E4M3, device=w.device)
+        scales = torch.empty(*w.shape[:-2], _blocks(n), _blocks(k), dtype=torch.float32, device=w.device)
+        load().quantize_blocks(w.data_ptr(), pitch(w), w.stride(0) if w.dim() == 3 else 0, q.data_ptr(), scales.data_ptr(), experts, n, k,
+                               ELEMS[w.dtype], stream_handle(index))
     return q, scales
 
 
@@ -78,14 +78,16 @@ def _tile_columns(rows, groups, n):
 def _check(a, sa, w, sw, offsets, out, dims):
     check_matrix(w, 'w', (_E4M3,), 16, dims=dims)
     n, k = w.shape[-2:]
-    check(n > 0 and n % 8 == 0, f'the rows of a weight must be a positive multiple of 8 (got {n})')
+    if n <= 0 or n % 8:
+        raise ValueError(f'the rows of a weight must be a positive multiple of 8 (got {n})')
     check_matrix(a, 'a', (_E4M3,), 16)
-    check(a.shape[1] == k, f'inner dimensions differ (a {a.shape[1]}, w {k})')
-    check(sa.dtype == torch.float32 and sa.shape == (a.shape[0], _blocks(k)) and all(s >= 0 for s in sa.stride()),
-          f'the scales of a must be float32 [{a.shape[0]}, {_blocks(k)}] (got {sa.dtype} {list(sa.shape)})')
+    if a.shape[1] != k:
+        raise ValueError(f'inner dimensions differ (a {a.shape[1]}, w {k})')
+    if sa.dtype != torch.float32 or sa.shape != (a.shape[0], _blocks(k)):
+        raise ValueError(f'the scales of a must be float32 [{a.shape[0]}, {_blocks(k)}] (got {sa.dtype} {list(sa.shape)})')
     want = (*w.shape[:-2], _blocks(n), _blocks(k))
-    check(sw.dtype == torch.float32 and sw.shape == want and sw.is_contiguous(),
-          f'the scales of w must be contiguous float32 {list(want)} (got {sw.dtype} {list(sw.shape)})')
+    if sw.dtype != torch.float32 or sw.shape != want or not sw.is_contiguous():
+        raise ValueError(f'the scales of w must be contiguous float32 {list(want)} (got {sw.dtype} {list(sw.shape)})')
     if offsets is not None:
         check(1 <= w.shape[0] <= MAX_EXPERTS, f'between 1 and {MAX_EXPERTS} experts are supported (got {w.shape[0]})')
         check_offsets(offsets, w.shape[0])
@@ -97,18 +99,18 @@ def _check(a, sa, w, sw, offsets, out, dims):
 
 
 def _product(a, sa, w, sw, offsets, out, stream, dims):
-    device = _check(a, sa, w, sw, offsets, out, dims)
-    with on_stream(device, stream, *(t for t in (a, sa, w, sw, offsets, out) if t is not None)):
+    index = _check(a, sa, w, sw, offsets, out, dims)
+    with on_stream(index, stream, (a, sa, w, sw, offsets, out)):
         rows, (n, k) = a.shape[0], w.shape[-2:]
         groups = w.shape[0] if dims == 3 else 1
         zero_rest = out is None and offsets is not None
         if out is None:
-            out = torch.empty(rows, n, dtype=torch.bfloat16, device=device)
+            out = torch.empty(rows, n, dtype=torch.bfloat16, device=a.device)
         if rows:
-            load().fp8_block_gemm(a.data_ptr(), pitch(a), sa.data_ptr(), sa.stride(0), sa.stride(1), w.data_ptr(), pitch(w),
-                                  w.stride(0) if groups > 1 else n * pitch(w), sw.data_ptr(), 0 if offsets is None else offsets.data_ptr(),
+            load().fp8_block_gemm(a.data_ptr(), pitch(a), sa.data_ptr(), *sa.stride(), w.data_ptr(), pitch(w),
+                                  matrix_stride(w) if dims == 3 else n * pitch(w), sw.data_ptr(), 0 if offsets is None else offsets.data_ptr(),
                                   out.data_ptr(), pitch(out), rows, groups, n, k, _tile_columns(rows, groups, n), rows <= 32, zero_rest,
-                                  error_words(device), stream_handle())
+                                  error_words(index), stream_handle(index))
     return out
 
 

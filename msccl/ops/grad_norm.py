@@ -42,13 +42,13 @@ def grad_norm(gradients, stream=None):
     in an order that depends on the sizes only."""
     tensors, gradients, _ = _collect(gradients, None)
     device = gradients[0].device
-    with on_stream(device, stream, *(gradients if stream is not None else ())):
+    with on_stream(device.index, stream, gradients):
         norm = torch.empty((), dtype=torch.float32, device=device)
         if len(tensors) == 0:
             return norm.zero_()
         partials = torch.empty(tensors.partials(), dtype=torch.float64, device=device)
-        load().grad_norm(tensors, partials.data_ptr(), stream_handle())
-        load().grad_sum(partials.data_ptr(), partials.numel(), 0, norm.data_ptr(), stream_handle())
+        load().grad_norm(tensors, partials.data_ptr(), stream_handle(device.index))
+        load().grad_sum(partials.data_ptr(), partials.numel(), 0, norm.data_ptr(), stream_handle(device.index))
     return norm
 
 
@@ -66,23 +66,23 @@ def clip_grad_norm(gradients, max_norm, out=None, reduce=None, stream=None):
     if tensors.overlapping():
         raise ValueError('a tensor that is written shares memory with another one')
     device = gradients[0].device
-    with on_stream(device, stream, *(gradients + (out or []) if stream is not None else ())):
+    with on_stream(device.index, stream, gradients + (out or [])):
         norm = torch.empty((), dtype=torch.float32, device=device)
         if len(tensors) == 0 and reduce is None:
             return norm.zero_()
         partials = torch.empty(max(tensors.partials(), 1), dtype=torch.float64, device=device)
         if len(tensors):
-            load().grad_norm(tensors, partials.data_ptr(), stream_handle())
+            load().grad_norm(tensors, partials.data_ptr(), stream_handle(device.index))
         else:
             partials.zero_()
         count = partials.numel()
         if reduce is not None:
             total = torch.empty(1, dtype=torch.float64, device=device)
-            load().grad_sum(partials.data_ptr(), count, total.data_ptr(), 0, stream_handle())
+            load().grad_sum(partials.data_ptr(), count, total.data_ptr(), 0, stream_handle(device.index))
             reduce(total)
             partials, count = total, 1
         if len(tensors):
-            load().grad_scale(tensors, partials.data_ptr(), count, max_norm, norm.data_ptr(), stream_handle())
+            load().grad_scale(tensors, partials.data_ptr(), count, max_norm, norm.data_ptr(), stream_handle(device.index))
         else:
-            load().grad_sum(partials.data_ptr(), count, 0, norm.data_ptr(), stream_handle())
+            load().grad_sum(partials.data_ptr(), count, 0, norm.data_ptr(), stream_handle(device.index))
     return norm

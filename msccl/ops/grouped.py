@@ -8,8 +8,8 @@ maximum.  Rows that belong to no expert come out as zeros, or, in an ``out`` tha
 import torch
 from torch.autograd.function import once_differentiable
 
-from msccl.ops._launch import (ELEMS, check, check_apart, check_devices, check_matrix, check_offsets, error_words, on_stream, pitch,
-                               stream_handle)
+from msccl.ops._launch import (ELEMS, check, check_apart, check_devices, check_matrix, check_offsets, error_words, matrix_stride, on_stream,
+                               pitch, stream_handle)
 from msccl.ops.moe_rows import MAX_EXPERTS, _kernel_rows
 from msccl.runtime.native import load
 
@@ -22,7 +22,8 @@ def _tile_rows(rows, experts):
 
 
 def _check_experts(experts):
-    check(1 <= experts <= MAX_EXPERTS, f'between 1 and {MAX_EXPERTS} experts are supported (got {experts})')
+    if not 1 <= experts <= MAX_EXPERTS:
+        raise ValueError(f'between 1 and {MAX_EXPERTS} experts are supported (got {experts})')
 
 
 def _product(x, w, offsets, out, backward):
@@ -31,10 +32,11 @@ def _product(x, w, offsets, out, backward):
     given = out is not None
     if not given:
         out = torch.empty(x.shape[0], columns, dtype=x.dtype, device=x.device)
-    if x.shape[0]:
-        load().grouped_gemm(x.data_ptr(), pitch(x), w.data_ptr(), pitch(w), w.stride(0) if experts > 1 else n * pitch(w), offsets.data_ptr(),
-                            out.data_ptr(), pitch(out), x.shape[0], experts, n, k, backward, ELEMS[x.dtype],
-                            _tile_rows(x.shape[0], experts), not given, error_words(x.device), stream_handle())
+    rows, index = x.shape[0], x.get_device()
+    if rows:
+        load().grouped_gemm(x.data_ptr(), pitch(x), w.data_ptr(), pitch(w), matrix_stride(w), offsets.data_ptr(), out.data_ptr(), pitch(out),
+                            rows, experts, n, k, backward, ELEMS[x.dtype], _tile_rows(rows, experts), not given, error_words(index),
+                            stream_handle(index))
     return out
 
 
@@ -44,9 +46,9 @@ def _weight_gradient(dy, x, offsets, out=None, dtype=None):
         out = torch.empty(experts, n, k, dtype=dtype or x.dtype, device=x.device)
     if x.shape[0] == 0:
         return out.zero_()
-    load().grouped_wgrad(dy.data_ptr(), pitch(dy), x.data_ptr(), pitch(x), offsets.data_ptr(), out.data_ptr(), pitch(out),
-                         out.stride(0) if experts > 1 else n * pitch(out), x.shape[0], experts, n, k, ELEMS[x.dtype],
-                         out.dtype == torch.float32, error_words(x.device), stream_handle())
+    index = x.get_device()
+    load().grouped_wgrad(dy.data_ptr(), pitch(dy), x.data_ptr(), pitch(x), offsets.data_ptr(), out.data_ptr(), pitch(out), matrix_stride(out),
+                         x.shape[0], experts, n, k, ELEMS[x.dtype], out.dtype == torch.float32, error_words(index), stream_handle(index))
     return out
 
 
@@ -60,7 +62,7 @@ class _Grouped(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
-        with on_stream(dy.device, None):
+        with on_stream(dy.get_device(), None):
             dy = _kernel_rows(dy, x.dtype)
             dx = _product(dy, w, offsets, None, True) if ctx.needs_input_grad[0] else None
             dw = _weight_gradient(dy, x, offsets) if ctx.needs_input_grad[1] else None
@@ -72,9 +74,11 @@ def _check_product(x, name, w, offsets, out, backward):
     experts, n, k = w.shape
     width, columns = (n, k) if backward else (k, n)
     _check_experts(experts)
-    check(n > 0 and n % 8 == 0, f'both dimensions of a weight must be positive multiples of 8 (got {n})')
+    if n <= 0 or n % 8:
+        raise ValueError(f'both dimensions of a weight must be positive multiples of 8 (got {n})')
     check_matrix(x, name, (w.dtype,), 8)
-    check(x.shape[1] == width, f'{name} has {x.shape[1]} columns, the weights expect {width}')
+    if x.shape[1] != width:
+        raise ValueError(f'{name} has {x.shape[1]} columns, the weights expect {width}')
     check_offsets(offsets, experts)
     if out is not None:
         check_matrix(out, 'out', (w.dtype,), 8)
@@ -87,17 +91,17 @@ def grouped_gemm(x, w, offsets, out=None, stream=None):
     """``y[t] = w[e] @ x[t]`` for the rows ``t`` of every expert ``e``: ``x`` [rows, k], ``w`` [experts, n, k] (both bf16 or both fp16,
     n and k multiples of 8, rows contiguous), result [rows, n] of the same type, fp32 sums.  Differentiable in ``x`` and ``w``; with
     ``out`` the result has no gradient."""
-    device = _check_product(x, 'x', w, offsets, out, False)
+    index = _check_product(x, 'x', w, offsets, out, False)
     needs = torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
     check(out is None or not needs, 'a result written to out has no gradient: detach x and w, or leave out away')
-    with on_stream(device, stream, x, w, offsets, *(() if out is None else (out,))):
+    with on_stream(index, stream, (x, w, offsets, out)):
         return _Grouped.apply(x, w, offsets) if needs else _product(x, w, offsets, out, False)
 
 
 def grouped_gemm_dgrad(dy, w, offsets, out=None, stream=None):
     """``dx[t] = w[e].T @ dy[t]``: ``dy`` [rows, n], ``w`` [experts, n, k], result [rows, k].  No gradient of its own."""
-    device = _check_product(dy, 'dy', w, offsets, out, True)
-    with on_stream(device, stream, dy, w, offsets, *(() if out is None else (out,))), torch.no_grad():
+    index = _check_product(dy, 'dy', w, offsets, out, True)
+    with on_stream(index, stream, (dy, w, offsets, out)):
         return _product(dy, w, offsets, out, True)
 
 
@@ -116,6 +120,6 @@ def grouped_gemm_wgrad(dy, x, offsets, out=None, dtype=None, stream=None):
         check(out.shape == (experts, dy.shape[1], x.shape[1]) and dtype in (None, out.dtype),
               f'out must be [{experts}, {dy.shape[1]}, {x.shape[1]}] of the type asked for')
         check_apart(out, dy=dy, x=x)
-    device = check_devices(dy=dy, x=x, offsets=offsets, out=out)
-    with on_stream(device, stream, dy, x, offsets, *(() if out is None else (out,))), torch.no_grad():
+    index = check_devices(dy=dy, x=x, offsets=offsets, out=out)
+    with on_stream(index, stream, (dy, x, offsets, out)):
         return _weight_gradient(dy, x, offsets, out, dtype)

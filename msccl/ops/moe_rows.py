@@ -12,7 +12,7 @@ from typing import NamedTuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from msccl.ops._launch import ELEMS, check, check_devices, check_matrix, on_stream, pitch, stream_handle
+from msccl.ops._launch import ELEMS, check_devices, check_matrix, on_stream, pitch, stream_handle
 from msccl.runtime.native import load
 
 MAX_EXPERTS, MAX_TOPK, MAX_COPIES = 512, 8, 1 << 22
@@ -30,23 +30,26 @@ class CopyOrder(NamedTuple):
 def sort_copies(experts, num_experts, stream=None):
     """Stable order of the copies ``experts`` [tokens, k] (int32 or int64) by expert, in one launch.  A copy whose id is outside
     ``[0, num_experts)`` is dropped: the gather gives it a row of zeros behind the last expert's, the combination ignores it."""
-    check(experts.dim() == 2 and experts.dtype in (torch.int32, torch.int64), 'experts must be a [tokens, k] int32 or int64 tensor')
+    if experts.dim() != 2 or experts.dtype not in (torch.int32, torch.int64):
+        raise ValueError('experts must be a [tokens, k] int32 or int64 tensor')
     tokens, topk = experts.shape
-    check(tokens >= 1 and 1 <= topk <= MAX_TOPK and tokens * topk <= MAX_COPIES,
-          f'sort_copies needs at least one token, k <= {MAX_TOPK} and at most {MAX_COPIES} copies (got {tokens} x {topk})')
-    check(1 <= num_experts <= MAX_EXPERTS, f'num_experts must be within 1 and {MAX_EXPERTS} (got {num_experts})')
-    with on_stream(check_devices(experts=experts), stream, experts):
+    copies = tokens * topk
+    if tokens < 1 or not 1 <= topk <= MAX_TOPK or copies > MAX_COPIES:
+        raise ValueError(f'sort_copies needs at least one token, k <= {MAX_TOPK} and at most {MAX_COPIES} copies (got {tokens} x {topk})')
+    if not 1 <= num_experts <= MAX_EXPERTS:
+        raise ValueError(f'num_experts must be within 1 and {MAX_EXPERTS} (got {num_experts})')
+    index = check_devices(experts=experts)
+    with on_stream(index, stream, (experts,)):
         experts = experts.contiguous()
-        copies = tokens * topk
         table = torch.empty(2 * copies + num_experts + 1, dtype=torch.int32, device=experts.device)
-        sorted_copy, position, offsets = table[:copies], table[copies:2 * copies], table[2 * copies:]
+        sorted_copy, position, offsets = table.split((copies, copies, num_experts + 1))
         load().sort_copies(experts.data_ptr(), experts.dtype == torch.int64, copies, num_experts, sorted_copy.data_ptr(),
-                           offsets.data_ptr(), position.data_ptr(), stream_handle())
+                           offsets.data_ptr(), position.data_ptr(), stream_handle(index))
     return CopyOrder(sorted_copy, offsets, position.view(tokens, topk))
 
 
 def _check_rows(t, name):
-    check_matrix(t, name, ELEMS, 16 // t.element_size())
+    check_matrix(t, name, ELEMS, 4 if t.dtype == torch.float32 else 8)
 
 
 def _rows_kept(order):
@@ -57,7 +60,7 @@ def _scatter(x, order):
     tokens, topk = order.position.shape
     out = torch.empty(tokens * topk, x.shape[1], dtype=x.dtype, device=x.device)
     load().scatter_rows(x.data_ptr(), pitch(x), out.data_ptr(), order.position.data_ptr(), _rows_kept(order), tokens, topk, x.shape[1],
-                        ELEMS[x.dtype], stream_handle())
+                        ELEMS[x.dtype], stream_handle(x.get_device()))
     return out
 
 
@@ -65,7 +68,7 @@ def _combine(ys, weights, order):
     tokens, topk = order.position.shape
     out = torch.empty(tokens, ys.shape[1], dtype=ys.dtype, device=ys.device)
     load().combine_rows(ys.data_ptr(), pitch(ys), 0 if weights is None else weights.data_ptr(), out.data_ptr(), order.position.data_ptr(),
-                        _rows_kept(order), tokens, topk, ys.shape[1], ELEMS[ys.dtype], stream_handle())
+                        _rows_kept(order), tokens, topk, ys.shape[1], ELEMS[ys.dtype], stream_handle(ys.get_device()))
     return out
 
 
@@ -87,7 +90,7 @@ class _Gather(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dxs):
-        with on_stream(dxs.device, None):
+        with on_stream(dxs.get_device(), None):
             return _combine(_kernel_rows(dxs, ctx.dtype), None, ctx.order), None
 
 
@@ -104,14 +107,14 @@ class _Combine(torch.autograd.Function):
         ys, weights = ctx.saved_tensors
         order = ctx.order
         tokens, topk = order.position.shape
-        with on_stream(dy.device, None):
+        with on_stream(dy.get_device(), None):
             dy = _kernel_rows(dy, ys.dtype)
             dys = torch.empty(ys.shape, dtype=ys.dtype, device=ys.device) if ctx.needs_input_grad[0] else None
             dweights = torch.empty(weights.shape, dtype=weights.dtype, device=ys.device) if ctx.needs_input_grad[1] else None
             load().combine_backward(dy.data_ptr(), pitch(dy), ys.data_ptr(), pitch(ys), weights.data_ptr(),
                                     0 if dys is None else dys.data_ptr(), 0 if dweights is None else dweights.data_ptr(),
                                     order.position.data_ptr(), _rows_kept(order), tokens, topk, ys.shape[1], ELEMS[ys.dtype],
-                                    stream_handle())
+                                    stream_handle(ys.get_device()))
         return dys, dweights, None
 
 
@@ -121,8 +124,9 @@ def gather_rows(x, order, stream=None):
     (fp32, in the order of ``j``, rounded once)."""
     _check_rows(x, 'x')
     tokens = order.position.shape[0]
-    check(x.shape[0] == tokens, f'x has {x.shape[0]} rows, the order {tokens} tokens')
-    with on_stream(check_devices(x=x, order=order.position), stream, x, order.position):
+    if x.shape[0] != tokens:
+        raise ValueError(f'x has {x.shape[0]} rows, the order {tokens} tokens')
+    with on_stream(check_devices(x=x, order=order.position), stream, (x, order.position)):
         return _Gather.apply(x, order) if torch.is_grad_enabled() and x.requires_grad else _scatter(x, order)
 
 
@@ -132,9 +136,11 @@ def combine_rows(ys, weights, order, stream=None):
     Gradients: ``ys`` and ``weights`` (zero for dropped copies)."""
     _check_rows(ys, 'ys')
     tokens, topk = order.position.shape
-    check(ys.shape[0] == tokens * topk, f'ys has {ys.shape[0]} rows, the order {tokens * topk} copies')
-    check(weights.dtype == torch.float32 and weights.shape == (tokens, topk), f'weights must be a [{tokens}, {topk}] float32 tensor')
-    with on_stream(check_devices(ys=ys, weights=weights, order=order.position), stream, ys, weights, order.position):
+    if ys.shape[0] != tokens * topk:
+        raise ValueError(f'ys has {ys.shape[0]} rows, the order {tokens * topk} copies')
+    if weights.dtype != torch.float32 or weights.shape != (tokens, topk):
+        raise ValueError(f'weights must be a [{tokens}, {topk}] float32 tensor')
+    with on_stream(check_devices(ys=ys, weights=weights, order=order.position), stream, (ys, weights, order.position)):
         weights = weights.contiguous()
         needs = torch.is_grad_enabled() and (ys.requires_grad or weights.requires_grad)
         return _Combine.apply(ys, weights, order) if needs else _combine(ys, weights, order)
