@@ -218,10 +218,24 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       float2 sum[COLS / 2];
 #pragma unroll
       for (int i = 0; i < COLS / 2; ++i) sum[i] = make_float2(0.0f, 0.0f);
-      float next = left > 0 ? sa[0] * sb[0] : 0.0f;
+      // scales two blocks ahead of their use, and multiplied only then: a load from L2 takes longer than a block
+      float a0 = 0.0f, b0 = 0.0f, a1 = 0.0f, b1 = 0.0f;
+      if (left > 0) {
+        a0 = sa[0];
+        b0 = sb[0];
+        if (k_blocks > 1) {
+          a1 = sa[g.sa_block];
+          b1 = sb[1];
+        }
+      }
       for (int kb = 0; kb < k_blocks; ++kb) {
-        const float scale = next;
-        if (left > 0 && kb + 1 < k_blocks) next = sa[(kb + 1) * g.sa_block] * sb[kb + 1];
+        const float scale = a0 * b0;
+        a0 = a1;
+        b0 = b1;
+        if (left > 0 && kb + 2 < k_blocks) {
+          a1 = sa[(kb + 2) * g.sa_block];
+          b1 = sb[kb + 2];
+        }
         ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag);
         ok = __all_sync(kFullMask, ok);
         if (!ok) {

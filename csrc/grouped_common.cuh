@@ -96,6 +96,34 @@ __device__ __forceinline__ uint32_t pack_16bit(bool bf16, float lo, float hi) {
   return r;
 }
 
+// An accumulator chunk with a feature per lane and 32 rows in the registers, as 16-bit values with eight features of one row per
+// lane: v[m] = features (lane & ~7) .. + 7 of row 8 m + lane % 8.  Three exchanges among eight lanes, 32 shuffles.  Four lanes then
+// store 64 consecutive bytes of a row; storing a register at a time would write 2 bytes per lane.
+template <bool BF16>
+__device__ __forceinline__ void transpose_chunk(const uint32_t (&r)[32], int lane, uint4 (&v)[4]) {
+  uint32_t s[16];                                // a pair of features, row 2 i + bit 0 of the lane
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t p = pack_16bit(BF16, __uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+    const uint32_t q = __shfl_xor_sync(kFullMask, p, 1);
+    s[i] = (lane & 1) ? __byte_perm(q, p, 0x7632) : __byte_perm(p, q, 0x5410);
+  }
+  uint2 u[8];                                    // four features, row 4 j + two bits of the lane
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool up = (lane & 2) != 0;
+    const uint32_t got = __shfl_xor_sync(kFullMask, up ? s[2 * j] : s[2 * j + 1], 2);
+    u[j] = up ? make_uint2(got, s[2 * j + 1]) : make_uint2(s[2 * j], got);
+  }
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    const bool up = (lane & 4) != 0;
+    const uint2 give = up ? u[2 * m] : u[2 * m + 1];
+    const uint2 got = make_uint2(__shfl_xor_sync(kFullMask, give.x, 4), __shfl_xor_sync(kFullMask, give.y, 4));
+    v[m] = up ? make_uint4(got.x, got.y, u[2 * m + 1].x, u[2 * m + 1].y) : make_uint4(u[2 * m].x, u[2 * m].y, got.x, got.y);
+  }
+}
+
 // A producer that gave up lets the loads that it issued land before shared memory is released (they take microseconds).
 __device__ __forceinline__ void drain_wait() {
   unsigned long long t0, t1;

@@ -11,8 +11,7 @@
 // streams the weights through tiles of 32 rows.  Rows of a tile that belong to the next group only reach columns of the accumulator
 // that are not stored, whatever they hold.  What is left of both operands behind the reduction dimension reads as zero.
 //
-// The accumulator holds a feature per lane and a row per column; the epilogue transposes 8 x 8 values among eight lanes with shuffles,
-// so that a lane stores 16 bytes of one row and four lanes store 64 consecutive bytes.
+// The accumulator holds a feature per lane and a row per column; the epilogue transposes it (transpose_chunk).
 //
 // Synchronisation is that of gemm_2cta_sm100.cu.
 #include <cuda.h>
@@ -199,31 +198,12 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         uint32_t r[32];
         tmem_ld32(taddr + c, r);
         tc_wait_ld();
-        // 1: (feature pair, row 2 i + bit 0 of the lane)
-        uint32_t s[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t p = pack_16bit(BF16, __uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-          const uint32_t q = __shfl_xor_sync(kFullMask, p, 1);
-          s[i] = (lane & 1) ? __byte_perm(q, p, 0x7632) : __byte_perm(p, q, 0x5410);
-        }
-        // 2: four features, row 4 j + two bits of the lane
-        uint2 u[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool up = (lane & 2) != 0;
-          const uint32_t got = __shfl_xor_sync(kFullMask, up ? s[2 * j] : s[2 * j + 1], 2);
-          u[j] = up ? make_uint2(got, s[2 * j + 1]) : make_uint2(s[2 * j], got);
-        }
-        // 3: eight features, row 8 m + three bits of the lane
+        uint4 v[4];
+        transpose_chunk<BF16>(r, lane, v);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          const bool up = (lane & 4) != 0;
-          const uint2 give = up ? u[2 * m] : u[2 * m + 1];
-          const uint2 got = make_uint2(__shfl_xor_sync(kFullMask, give.x, 4), __shfl_xor_sync(kFullMask, give.y, 4));
-          const uint4 v = up ? make_uint4(got.x, got.y, u[2 * m + 1].x, u[2 * m + 1].y) : make_uint4(u[2 * m].x, u[2 * m].y, got.x, got.y);
           const int t = c + 8 * m + (lane & 7);
-          if (in && t < columns) *reinterpret_cast<uint4*>(g.out + (row + t) * g.ldo + f) = v;
+          if (in && t < columns) *reinterpret_cast<uint4*>(g.out + (row + t) * g.ldo + f) = v[m];
         }
       }
       tc_fence_before_sync();
