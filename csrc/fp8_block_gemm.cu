@@ -10,6 +10,9 @@
 // a row, so that one number per thread and block scales all of its columns.  Tiles are 128 rows x BN columns of one CTA: warps
 // 2 .. 9 take a quarter of the rows and half of the columns each.
 //
+// The operands of a 128 x 256 tile would take more of L2 than an SM gets (48 KB per block of K), so large products run on CTA pairs
+// (fp8_block_2cta.cu); this kernel has the tiles of up to 128 columns that small ones need to fill the GPU.
+//
 // With at most 32 rows in every tile only 32 rows of `a` are loaded; the tensor core then reads whatever follows in shared memory
 // as the other rows (still inside the allocation) and their results are not read.
 //
@@ -21,6 +24,7 @@
 #include "expert_ops.h"
 #include "gemm_sm100.cuh"
 #include "gemm_sm100.h"
+#include "fp8_block.cuh"
 #include "grouped_common.cuh"
 
 namespace msccl {
@@ -30,8 +34,6 @@ namespace {
 
 constexpr int kFThreads = 320;                   // 0 producer, 1 MMA, 2..9 scaling and epilogue
 constexpr int kFEpilogueWarps = 8;
-constexpr int kFBlock = 128;                     // K values per scale = bytes per shared-memory row
-constexpr int kFGroupTileRows = 2048;
 constexpr int kFSmemLimit = 216 * 1024;
 
 template <int BN, int AR> struct FGeometry {
@@ -44,17 +46,6 @@ template <int BN, int AR> struct FGeometry {
   static constexpr int kAccs = 512 / BN < 4 ? 512 / BN : 4;
   static constexpr int kTmemCols = kAccs * BN;
   static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStageBytes + kBehind + 512;
-};
-
-struct FArgs {
-  const int* offsets;                            // nullptr: one group of all rows
-  const float *sa, *sb;
-  long long sa_row, sa_block;                    // strides of sa
-  __nv_bfloat16* out;
-  long long ldo;
-  int rows, groups, n, k;
-  int zero_rest;
-  int* error_words;
 };
 
 __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
@@ -73,16 +64,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
-// Two fp32 sums at once: acc += scale * v.
-__device__ __forceinline__ void fma2(float2& acc, float2 scale, uint32_t lo, uint32_t hi) {
-  unsigned long long a, s, v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(acc.x), "f"(acc.y));
-  asm("mov.b64 %0, {%1, %2};" : "=l"(s) : "f"(scale.x), "f"(scale.y));
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(s), "l"(v));
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(acc.x), "=f"(acc.y) : "l"(a));
-}
-
 template <int BN, int AR>
 __global__ void __launch_bounds__(kFThreads, 1)
 fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const FArgs g) {
@@ -119,16 +100,7 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     prefetch_tensormap(&map_w);
   }
   if (warp == 1) tmem_alloc(tmem_slot, Geo::kTmemCols);
-  if (warp == 2) {
-    auto tiles_of = [&](int rows) { return (rows + BM - 1) / BM * n_tiles; };
-    if (g.offsets != nullptr) {
-      build_groups(table, g.offsets, g.groups, g.rows, tiles_of);
-    } else if (lane == 0) {
-      table.row_start[0] = table.tile_start[0] = 0;
-      table.row_start[1] = g.rows;
-      table.tile_start[1] = tiles_of(g.rows);
-    }
-  }
+  if (warp == 2) build_table(table, g, [&](int rows) { return (rows + BM - 1) / BM * n_tiles; });
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -212,30 +184,12 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       const int left = table.row_start[e + 1] - row - quarter * 32;       // rows of this warp that are the group's
       row += quarter * 32 + lane;
       column += half * COLS;
-      const float* sa = g.sa + min(row, g.rows - 1) * g.sa_row;
-      const int sb_rows = (g.n + kFBlock - 1) / kFBlock;
-      const float* sb = g.sb + (static_cast<long long>(e) * sb_rows + min(column / kFBlock, sb_rows - 1)) * k_blocks;
       float2 sum[COLS / 2];
 #pragma unroll
       for (int i = 0; i < COLS / 2; ++i) sum[i] = make_float2(0.0f, 0.0f);
-      // scales two blocks ahead of their use, and multiplied only then: a load from L2 takes longer than a block
-      float a0 = 0.0f, b0 = 0.0f, a1 = 0.0f, b1 = 0.0f;
-      if (left > 0) {
-        a0 = sa[0];
-        b0 = sb[0];
-        if (k_blocks > 1) {
-          a1 = sa[g.sa_block];
-          b1 = sb[1];
-        }
-      }
+      ScaleStream scales(g.sa + min(row, g.rows - 1) * g.sa_row, g.sa_block, weight_scales(g, e, column, k_blocks), k_blocks, left > 0);
       for (int kb = 0; kb < k_blocks; ++kb) {
-        const float scale = a0 * b0;
-        a0 = a1;
-        b0 = b1;
-        if (left > 0 && kb + 2 < k_blocks) {
-          a1 = sa[(kb + 2) * g.sa_block];
-          b1 = sb[kb + 2];
-        }
+        const float scale = scales.next();
         ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag);
         ok = __all_sync(kFullMask, ok);
         if (!ok) {
@@ -251,7 +205,7 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             if constexpr (CHUNK == 32) {
               uint32_t r[32];
               tmem_ld32(taddr + c, r);
-              tc_wait_ld();
+              wait_loaded(r);
 #pragma unroll
               for (int i = 0; i < 16; ++i) fma2(sum[c / 2 + i], s2, r[2 * i], r[2 * i + 1]);
             } else {
@@ -268,23 +222,9 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         if (lane == 0) mbar_arrive(&acc_empty[acc]);
         if (++acc == ACCS) { acc = 0; acc_phase ^= 1; }
       }
-      if (ok && lane < left) {
-        __nv_bfloat16* out = g.out + row * g.ldo + column;
-#pragma unroll
-        for (int c = 0; c < COLS; c += 8)
-          if (column + c < g.n)
-            *reinterpret_cast<uint4*>(out + c) = make_uint4(pack_bf16(sum[c / 2].x, sum[c / 2].y), pack_bf16(sum[c / 2 + 1].x, sum[c / 2 + 1].y),
-                                                            pack_bf16(sum[c / 2 + 2].x, sum[c / 2 + 2].y), pack_bf16(sum[c / 2 + 3].x, sum[c / 2 + 3].y));
-      }
+      if (ok && lane < left) store_row(g, row, column, sum);
     }
-    if (g.zero_rest && !skip) {
-      const int head = table.row_start[0], tail = table.row_start[g.groups];
-      const int rest = head + g.rows - tail;
-      for (int i = blockIdx.x * kFEpilogueWarps + warp - 2; i < rest; i += gridDim.x * kFEpilogueWarps) {
-        uint4* dst = reinterpret_cast<uint4*>(g.out + static_cast<long long>(i < head ? i : tail + i - head) * g.ldo);
-        for (int v = lane; v < g.n / 8; v += 32) dst[v] = make_uint4(0, 0, 0, 0);
-      }
-    }
+    if (g.zero_rest && !skip) zero_rest_rows(table, g, blockIdx.x * kFEpilogueWarps + warp - 2, gridDim.x * kFEpilogueWarps);
   }
 
   tc_fence_before_sync();
@@ -316,7 +256,7 @@ cudaError_t launch(const CUtensorMap& map_a, const CUtensorMap& map_w, const FAr
 
 // a: [rows, k] e4m3 (pitch lda bytes), sa: [rows, ceil(k / 128)] with the strides given; w: [groups, n, k] e4m3 (pitch ldw, matrix
 // stride lde), sb: [groups, ceil(n / 128), ceil(k / 128)] contiguous; out: [rows, n] bf16.  k % 16 == 0, n % 8 == 0.
-// bn: 32, 64, 128 or 256; few_rows: no group has more than 32 rows.
+// bn: 32, 64 or 128 (columns per tile of one CTA), or 256: the CTA-pair kernel; few_rows: no group has more than 32 rows.
 cudaError_t launch_fp8_block_gemm(const void* a, long long lda, const float* sa, long long sa_row, long long sa_block, const void* w,
                                   long long ldw, long long lde, const float* sb, const int* offsets, void* out, long long ldo, int rows,
                                   int groups, int n, int k, int bn, bool few_rows, bool zero_rest, int* error_words, cudaStream_t stream) {
@@ -338,20 +278,22 @@ cudaError_t launch_fp8_block_gemm(const void* a, long long lda, const float* sa,
   g.zero_rest = zero_rest ? 1 : 0;
   g.error_words = error_words;
   const uint64_t a_dims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(rows)}, a_strides[1] = {static_cast<uint64_t>(lda)};
+  if (bn == 256) few_rows = false;
   const uint32_t a_box[2] = {kFBlock, few_rows ? 32u : static_cast<uint32_t>(BM)};
   const CUtensorMap map_a = make_swizzled_map(a, 1, 2, a_dims, a_strides, a_box);
   const uint64_t w_dims[3] = {static_cast<uint64_t>(k), static_cast<uint64_t>(n), static_cast<uint64_t>(groups)};
   const uint64_t w_strides[2] = {static_cast<uint64_t>(ldw), static_cast<uint64_t>(lde)};
-  const uint32_t w_box[3] = {kFBlock, static_cast<uint32_t>(bn), 1};
+  const uint32_t w_box[3] = {kFBlock, static_cast<uint32_t>(bn == 256 ? bn / 2 : bn), 1};
   const CUtensorMap map_w = make_swizzled_map(w, 1, 3, w_dims, w_strides, w_box);
-  const long long active = groups < rows ? groups : rows, most = static_cast<long long>((n + bn - 1) / bn) * (rows / BM + active);
+  const int tile_rows = bn == 256 ? 2 * BM : BM;
+  const long long active = groups < rows ? groups : rows, most = static_cast<long long>((n + bn - 1) / bn) * (rows / tile_rows + active);
   if (most > (1ll << 30)) return cudaErrorInvalidValue;
   const int tiles = static_cast<int>(most);
   switch (bn) {
     case 32: return few_rows ? launch<32, 32>(map_a, map_w, g, tiles, stream) : launch<32, BM>(map_a, map_w, g, tiles, stream);
     case 64: return few_rows ? launch<64, 32>(map_a, map_w, g, tiles, stream) : launch<64, BM>(map_a, map_w, g, tiles, stream);
     case 128: return few_rows ? launch<128, 32>(map_a, map_w, g, tiles, stream) : launch<128, BM>(map_a, map_w, g, tiles, stream);
-    case 256: return few_rows ? launch<256, 32>(map_a, map_w, g, tiles, stream) : launch<256, BM>(map_a, map_w, g, tiles, stream);
+    case 256: return launch_fp8_block_pairs(map_a, map_w, g, tiles, stream);
     default: return cudaErrorInvalidValue;
   }
 }

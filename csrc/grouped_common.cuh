@@ -71,6 +71,12 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
+// Arrival on a barrier of the pair that orders no memory of this thread: an accumulator is free once its loads have returned
+// (tcgen05.wait::ld).  The releasing form waits until the thread's stores are visible to the cluster, half a microsecond and more.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // Operand whose M (or N) dimension is the contiguous one, 128-byte swizzle: slabs of 64 elements x 64 reduction rows (8 KB, 128
 // bytes per reduction row).  Leading byte offset: from one slab to the next; stride byte offset: 8 reduction rows.
 constexpr int kSlabBytes = 64 * 128;
@@ -94,6 +100,17 @@ __device__ __forceinline__ uint32_t pack_16bit(bool bf16, float lo, float hi) {
   if (bf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// Wait for this thread's tensor-memory loads; the registers pass through, so that nothing that uses them moves ahead of the wait.
+__device__ __forceinline__ void wait_loaded(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :: "memory");
+  asm volatile("" : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :: "memory");
 }
 
 // An accumulator chunk with a feature per lane and 32 rows in the registers, as 16-bit values with eight features of one row per

@@ -31,6 +31,8 @@ namespace sm100 {
 namespace {
 
 constexpr int kGroupTileRows = 2048;             // rows that a group of tiles walks together (L2, see tile_coords)
+constexpr int kGEpilogueWarps = 8;               // two on each quarter of the lanes; with four the transposition of a tile took 4.8 us
+constexpr int kGThreads = 64 + 32 * kGEpilogueWarps;
 constexpr int kGABytes = BM * BK * 2;            // this CTA's 128 features: 16 KB
 constexpr int kGSmemLimit = 220 * 1024;
 
@@ -53,7 +55,7 @@ struct GroupedArgs {
 };
 
 template <int BN, bool MN_MAJOR, bool BF16>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(kGThreads, 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const GroupedArgs g) {
   using Geo = Geometry<BN>;
   constexpr int S = Geo::kStages;
@@ -82,7 +84,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 8);
+      mbar_init(&acc_empty[a], 2 * kGEpilogueWarps);
     }
     *abort_flag = 0;
     mbar_fence_init();
@@ -176,7 +178,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       }
     }
   } else {
-    const int quarter = warp % 4;
+    const int quarter = warp % 4, half = (warp - 2) / 4;      // the halves take every other chunk of 32 columns
     int acc = 0, e = 0;
     uint32_t acc_phase = 0;
     for (int tile = first; tile < num_tiles; tile += step) {
@@ -194,10 +196,10 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       const int f = feature + static_cast<int>(rank) * BM + quarter * 32 + (lane & ~7);       // this lane stores features f .. f + 7
       const bool in = f < g.features;
       const int columns = min(BN, row_end - row);
-      for (int c = 0; c < columns; c += 32) {
+      for (int c = half * 32; c < columns; c += 64) {
         uint32_t r[32];
         tmem_ld32(taddr + c, r);
-        tc_wait_ld();
+        wait_loaded(r);
         uint4 v[4];
         transpose_chunk<BF16>(r, lane, v);
 #pragma unroll
@@ -208,13 +210,13 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       }
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[acc]), 0));
+      if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&acc_empty[acc]), 0));
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
     if (g.zero_rest) {                           // rows before the first group and behind the last one
       const int head = table.row_start[0], tail = table.row_start[g.groups];
       const int rest = head + g.rows - tail;
-      for (int i = blockIdx.x * 4 + quarter; i < rest; i += gridDim.x * 4) {
+      for (int i = blockIdx.x * kGEpilogueWarps + warp - 2; i < rest; i += gridDim.x * kGEpilogueWarps) {
         uint4* dst = reinterpret_cast<uint4*>(g.out + static_cast<long long>(i < head ? i : tail + i - head) * g.ldo);
         for (int v = lane; v < g.features / 8; v += 32) dst[v] = make_uint4(0, 0, 0, 0);
       }
@@ -239,12 +241,12 @@ cudaError_t launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const Gro
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (cached[dev] == 0) {
     int clusters = 0;
-    err = pair_clusters(kernel, Geometry<BN>::kSmem, &clusters);
+    err = pair_clusters(kernel, Geometry<BN>::kSmem, &clusters, kGThreads);
     if (err != cudaSuccess) return err;
     if (clusters <= 0) return cudaErrorLaunchOutOfResources;
     cached[dev] = clusters;
   }
-  return launch_pairs(kernel, Geometry<BN>::kSmem, most_tiles < cached[dev] ? most_tiles : cached[dev], stream, map_w, map_x, g);
+  return launch_pairs_threads(kernel, Geometry<BN>::kSmem, most_tiles < cached[dev] ? most_tiles : cached[dev], kGThreads, stream, map_w, map_x, g);
 }
 
 template <int BN>

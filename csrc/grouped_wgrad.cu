@@ -17,6 +17,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "expert_ops.h"
 #include "gemm_sm100.cuh"
 #include "gemm_sm100.h"
@@ -28,7 +30,8 @@ namespace sm100 {
 
 namespace {
 
-constexpr int kWThreads = 224;                   // 0 producer, 1 MMA, 2..5 epilogue, 6 fix-up
+constexpr int kWEpilogueWarps = 4;
+constexpr int kWThreads = 96 + 32 * kWEpilogueWarps;      // 0 producer, 1 MMA, 2..5 epilogue, 6 fix-up
 constexpr int kWTile = 256;
 constexpr int kWOperand = 2 * kSlabBytes;        // 128 features x 64 rows
 constexpr int kWStageBytes = 2 * kWOperand;
@@ -75,7 +78,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 8);
+      mbar_init(&acc_empty[a], 2 * kWEpilogueWarps);
     }
     *abort_flag = 0;
     mbar_fence_init();
@@ -180,7 +183,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
     }
-  } else if (warp == 6) {
+  } else if (warp == 2 + kWEpilogueWarps) {
     int stage = 0;
     uint32_t tail_phase = 0;                     // one bit per stage
     for (int tile = first; tile < num_tiles; tile += step) {
@@ -223,10 +226,14 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
         }
         tc_fence_after_sync();
       }
-      const int k = k0 + static_cast<int>(rank) * BM + quarter * 32 + (F32OUT ? lane : lane & ~7);      // the first that this lane stores
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kWTile);
       const int columns = min(kWTile, g.n - n0);
-      const long long at = e * g.lde + n0 * g.ldo + k;
+      // fp32: a lane stores value k of row n0 + c + i; 16 bits: values k .. k + 7 of row n0 + c + 8 m + lane % 8
+      const int k = k0 + static_cast<int>(rank) * BM + quarter * 32 + (F32OUT ? lane : lane & ~7), lane_row = F32OUT ? 0 : lane & 7;
+      const bool in = k < g.k;
+      using Out = std::conditional_t<F32OUT, float, uint16_t>;
+      Out* dst = static_cast<Out*>(g.out) + e * g.lde + (n0 + lane_row) * g.ldo + k;
+      const long long row8 = 8 * g.ldo;
       for (int c = 0; c < columns; c += 32) {
         uint32_t r[32];
         if (empty) {
@@ -234,26 +241,29 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
           for (int i = 0; i < 32; ++i) r[i] = 0u;
         } else {
           tmem_ld32(taddr + c, r);
-          tc_wait_ld();
+          wait_loaded(r);
         }
-        if (F32OUT) {
+        const int left = in ? columns - c - lane_row : 0;      // rows from this lane's first on
+        if constexpr (F32OUT) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (k < g.k && c + i < columns) static_cast<float*>(g.out)[at + (c + i) * g.ldo] = __uint_as_float(r[i]);
+          for (int i = 0; i < 32; ++i) {
+            if (i < left) *dst = __uint_as_float(r[i]);
+            dst += g.ldo;
+          }
         } else {
           uint4 v[4];
           transpose_chunk<BF16>(r, lane, v);
 #pragma unroll
           for (int m = 0; m < 4; ++m) {
-            const int i = c + 8 * m + (lane & 7);
-            if (k < g.k && i < columns) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(g.out) + at + i * g.ldo) = v[m];
+            if (8 * m < left) *reinterpret_cast<uint4*>(dst) = v[m];
+            dst += row8;
           }
         }
       }
       if (!empty) {
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[acc]), 0));
+        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&acc_empty[acc]), 0));
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
     }
