@@ -119,7 +119,7 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   };
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       int stage = 0, e = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -142,7 +142,7 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       if (!ok) drain_wait();
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>(BM >> 4) << 24);   // e4m3 x e4m3 -> fp32
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
@@ -190,8 +190,7 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       ScaleStream scales(g.sa + min(row, g.rows - 1) * g.sa_row, g.sa_block, weight_scales(g, e, column, k_blocks), k_blocks, left > 0);
       for (int kb = 0; kb < k_blocks; ++kb) {
         const float scale = scales.next();
-        ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag);
-        ok = __all_sync(kFullMask, ok);
+        ok = mbar_wait_warp(&acc_full[acc], acc_phase, abort_flag);
         if (!ok) {
           if (lane == 0) gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 2, acc);
           break;
@@ -283,7 +282,7 @@ cudaError_t launch_fp8_block_gemm(const void* a, long long lda, const float* sa,
   const CUtensorMap map_a = make_swizzled_map(a, 1, 2, a_dims, a_strides, a_box);
   const uint64_t w_dims[3] = {static_cast<uint64_t>(k), static_cast<uint64_t>(n), static_cast<uint64_t>(groups)};
   const uint64_t w_strides[2] = {static_cast<uint64_t>(ldw), static_cast<uint64_t>(lde)};
-  const uint32_t w_box[3] = {kFBlock, static_cast<uint32_t>(bn == 256 ? bn / 2 : bn), 1};
+  const uint32_t w_box[3] = {kFBlock, static_cast<uint32_t>(bn == 256 ? 64 : bn), 1};
   const CUtensorMap map_w = make_swizzled_map(w, 1, 3, w_dims, w_strides, w_box);
   const int tile_rows = bn == 256 ? 2 * BM : BM;
   const long long active = groups < rows ? groups : rows, most = static_cast<long long>((n + bn - 1) / bn) * (rows / tile_rows + active);

@@ -22,9 +22,8 @@ struct GroupTable {
   int tile_start[kMaxGroups + 1];
 };
 
-// Whole warp.  tiles_of(rows) = tiles of a group of that many rows.
-template <typename TilesOf>
-__device__ __forceinline__ void build_groups(GroupTable& g, const int* __restrict__ offsets, int groups, int rows, TilesOf tiles_of) {
+// Whole warp.
+__device__ __forceinline__ void build_row_starts(int* row_start, const int* __restrict__ offsets, int groups, int rows) {
   const int lane = threadIdx.x % 32;
   int high = 0;                                  // running maximum
   for (int b = 0; b <= groups; b += 32) {
@@ -35,10 +34,17 @@ __device__ __forceinline__ void build_groups(GroupTable& g, const int* __restric
       const int up = __shfl_up_sync(kFullMask, v, off);
       if (lane >= off) v = max(v, up);
     }
-    if (b + lane <= groups) g.row_start[b + lane] = v;
+    if (b + lane <= groups) row_start[b + lane] = v;
     high = __shfl_sync(kFullMask, v, 31);
   }
   __syncwarp();
+}
+
+// Whole warp.  tiles_of(rows) = tiles of a group of that many rows.
+template <typename TilesOf>
+__device__ __forceinline__ void build_groups(GroupTable& g, const int* __restrict__ offsets, int groups, int rows, TilesOf tiles_of) {
+  const int lane = threadIdx.x % 32;
+  build_row_starts(g.row_start, offsets, groups, rows);
   int before = 0;
   if (lane == 0) g.tile_start[0] = 0;
   for (int b = 0; b < groups; b += 32) {
@@ -75,6 +81,39 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
 // (tcgen05.wait::ld).  The releasing form waits until the thread's stores are visible to the cluster, half a microsecond and more.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// One lane of a converged warp.  Code behind `if (elect_one())` is known to run in one thread: tcgen05.mma then costs 39 clocks to
+// issue and a commit about 5, against 54 and 44 behind `if (lane == 0)`.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// mbar_wait whose first polls neither suspend the thread nor read the clock: where the wait is on the critical path of every block of
+// K, waking up is too.
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+#pragma unroll 1
+  for (int i = 0; i < 256; ++i)
+    if (mbar_test_wait(bar, parity)) return true;
+  return mbar_wait(bar, parity, abort_flag);
+}
+
+// Wait of a whole warp: one lane polls for all.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  int ok = 1;
+  if (threadIdx.x % 32 == 0) ok = mbar_wait_soon(bar, parity, abort_flag) ? 1 : 0;
+  return __shfl_sync(kFullMask, ok, 0) != 0;
 }
 
 // Operand whose M (or N) dimension is the contiguous one, 128-byte swizzle: slabs of 64 elements x 64 reduction rows (8 KB, 128

@@ -113,7 +113,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   if (skip) {
     // fall through to the common exit
   } else if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       int stage = 0, e = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -144,7 +144,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       if (!ok) drain_wait();
     }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (leader && elect_one()) {
       constexpr uint32_t idesc = idesc_16bit(BF16, 2 * BM, BN) | (MN_MAJOR ? kIdescTransA : 0u);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
@@ -185,8 +185,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       int row, feature;
       locate(tile, e, row, feature);
       const int row_end = table.row_start[e + 1];
-      bool ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag);
-      ok = __all_sync(kFullMask, ok);
+      bool ok = mbar_wait_warp(&acc_full[acc], acc_phase, abort_flag);
       if (!ok) {
         if (lane == 0) gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 2, acc);
         break;

@@ -5,15 +5,16 @@
 // the lanes of an accumulator run along k, the contiguous dimension of the result (dy as the M operand gave every lane a row of
 // its own to store to, 16 bytes at a time: 8 groups of 1024 rows, n = k = 4096, 432 us).
 //
-// The reduction is ragged: the last 64-row block of a group also holds rows of the next group (or memory behind the last one,
-// which may hold anything).  Those rows have to be zero in both operands, since 0 times infinity is not 0.  Loading that block
-// completes on a barrier of the CTA's own instead of the leader's; a fix-up warp then clears the rows, orders its writes before
-// the tensor core's reads and tells the MMA thread.  All other blocks never pass through it.
+// The reduction is ragged: the last 64-row block of a group also covers rows of the next group (or memory behind the last one, which
+// may hold anything).  Those rows have to be zero in both operands, since 0 times infinity is not 0.  So that block goes a way of
+// its own: a fix-up warp in each CTA loads it into a buffer beside the pipeline, clears the rows, orders its writes before the tensor
+// core's reads and tells the MMA thread, which takes the block last.  The buffer is free again when the tile is done, so the block
+// of the next tile is ready long before its turn.  (Through the pipeline, every such block held up the tensor core for 1.5 us.)
 //
-//   tail_full[s]    one per CTA: this CTA's loads of a last block (full[s] then completes without bytes).
-//   tail_ready[s]   leader only, two arrivals: the fix-up warps of the pair.  The MMA thread waits for it before a last block.
-// The other barriers are those of gemm_2cta_sm100.cu.  An arrival of each producer on the leader's barrier with every block (in place
-// of tail_ready) releases memory at cluster scope and took 0.55 us of the 0.83 us per block.
+//   tail_full    one per CTA: this CTA's loads of the block.      tail_empty   one per CTA: its MMAs are done (commit).
+//   tail_ready   leader only, two arrivals: the fix-up warps of the pair.
+// The other barriers are those of gemm_2cta_sm100.cu.  An arrival of each producer on the leader's barrier with every block releases
+// memory at cluster scope and took 0.55 us of 0.83 us per block; nothing of that kind is in the loop.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -37,7 +38,10 @@ constexpr int kWOperand = 2 * kSlabBytes;        // 128 features x 64 rows
 constexpr int kWStageBytes = 2 * kWOperand;
 constexpr int kWStages = 6;
 constexpr int kWTmemCols = 2 * kWTile;
-constexpr size_t kWSmem = 1024 + static_cast<size_t>(kWStages) * kWStageBytes + 256;
+// the pipeline, the block on its own, row_start of the groups, the barriers: 226 KB, so the base has to be aligned as it is
+constexpr int kWTableBytes = (kMaxGroups + 1) * 4 + 12;
+constexpr size_t kWSmem = static_cast<size_t>(kWStages + 1) * kWStageBytes + kWTableBytes + 256;
+static_assert(kWSmem <= 227 * 1024 && kWTableBytes % 16 == 0, "");
 
 struct WgradArgs {
   const int* offsets;
@@ -51,15 +55,15 @@ template <bool BF16, bool F32OUT>
 __global__ void __launch_bounds__(kWThreads, 1)
 grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_x, const WgradArgs g) {
   constexpr int S = kWStages;
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ GroupTable table;
-  __shared__ int s_skip;
-  uint8_t* stage_base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(stage_base + static_cast<size_t>(S) * kWStageBytes);
-  uint64_t *full_bar = bars, *empty_bar = bars + S, *tail_full = bars + 2 * S, *tail_ready = bars + 3 * S;
-  uint64_t *acc_full = bars + 4 * S, *acc_empty = bars + 4 * S + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * S + 4);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  extern __shared__ __align__(1024) uint8_t stage_base[];
+  uint8_t* tail_base = stage_base + static_cast<size_t>(S) * kWStageBytes;
+  int* row_start = reinterpret_cast<int*>(tail_base + kWStageBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(row_start) + kWTableBytes);
+  uint64_t *full_bar = bars, *empty_bar = bars + S, *acc_full = bars + 2 * S, *acc_empty = bars + 2 * S + 2;
+  uint64_t *tail_full = bars + 2 * S + 4, *tail_ready = tail_full + 1, *tail_empty = tail_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 8);
+  int* s_skip = reinterpret_cast<int*>(tmem_slot + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cluster_ctarank();
@@ -69,29 +73,35 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
   const int per_group = n_tiles * k_tiles, num_tiles = per_group * g.groups;
 
   if (threadIdx.x == 0) {
-    s_skip = g.error_words != nullptr && *reinterpret_cast<volatile int*>(g.error_words) != 0 ? 1 : 0;
+    // an earlier launch gave up: skip the work; the leader's reading decides for the pair
+    *s_skip = g.error_words != nullptr && *reinterpret_cast<volatile int*>(g.error_words) != 0 ? 1 : 0;
     for (int s = 0; s < S; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
-      mbar_init(&tail_full[s], 1);
-      mbar_init(&tail_ready[s], 2);
     }
+    mbar_init(tail_full, 1);
+    mbar_init(tail_ready, 2);
+    mbar_init(tail_empty, 1);
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
       mbar_init(&acc_empty[a], 2 * kWEpilogueWarps);
     }
     *abort_flag = 0;
+    if (smem_u32(stage_base) % 1024 != 0) {        // the swizzle pattern starts on such a boundary: nothing would be right
+      *s_skip = 1;
+      gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_EMPTY, 9, 0);
+    }
     mbar_fence_init();
     prefetch_tensormap(&map_dy);
     prefetch_tensormap(&map_x);
   }
   if (warp == 1) tmem_alloc_pair(tmem_slot, kWTmemCols);
-  if (warp == 2) build_groups(table, g.offsets, g.groups, g.rows, [](int) { return 0; });
+  if (warp == 2) build_row_starts(row_start, g.offsets, g.groups, g.rows);
   tc_fence_before_sync();
   cluster_sync_all();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
-  const bool skip = ld_shared_cluster_u32(map_to_cta(smem_u32(&s_skip), 0)) != 0;
+  const bool skip = ld_shared_cluster_u32(map_to_cta(smem_u32(s_skip), 0)) != 0;
 
   auto locate = [&](int tile, int& e, int& n0, int& k0) {
     e = tile / per_group;
@@ -104,7 +114,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
   if (skip) {
     // fall through to the common exit
   } else if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -113,8 +123,8 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
         locate(tile, e, n0, k0);
         n0 += static_cast<int>(rank) * BM;
         k0 += static_cast<int>(rank) * BM;
-        const int lo = table.row_start[e], rows = table.row_start[e + 1] - lo;
-        for (int r = 0; r < rows; r += BK) {
+        const int lo = row_start[e], end = row_start[e + 1];
+        for (int r = lo; r + BK <= end; r += BK) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) {
             gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_EMPTY, 0, stage);
             ok = false;
@@ -122,33 +132,30 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
           }
           uint8_t* dst = stage_base + static_cast<size_t>(stage) * kWStageBytes;
           const uint32_t bar = map_to_cta(smem_u32(&full_bar[stage]), 0);
-          if (rows - r >= BK) {
-            if (leader) mbar_expect_tx(&full_bar[stage], 2 * kWStageBytes);
-            tma_pair_2d(dst, &map_x, bar, k0, lo + r);
-            tma_pair_2d(dst + kSlabBytes, &map_x, bar, k0 + 64, lo + r);
-            tma_pair_2d(dst + kWOperand, &map_dy, bar, n0, lo + r);
-            tma_pair_2d(dst + kWOperand + kSlabBytes, &map_dy, bar, n0 + 64, lo + r);
-          } else {
-            if (leader) mbar_arrive(&full_bar[stage]);
-            mbar_expect_tx(&tail_full[stage], kWStageBytes);
-            tma_load_2d(dst, &map_x, &tail_full[stage], k0, lo + r);
-            tma_load_2d(dst + kSlabBytes, &map_x, &tail_full[stage], k0 + 64, lo + r);
-            tma_load_2d(dst + kWOperand, &map_dy, &tail_full[stage], n0, lo + r);
-            tma_load_2d(dst + kWOperand + kSlabBytes, &map_dy, &tail_full[stage], n0 + 64, lo + r);
-          }
+          if (leader) mbar_expect_tx(&full_bar[stage], 2 * kWStageBytes);
+          tma_pair_2d(dst, &map_x, bar, k0, r);
+          tma_pair_2d(dst + kSlabBytes, &map_x, bar, k0 + 64, r);
+          tma_pair_2d(dst + kWOperand, &map_dy, bar, n0, r);
+          tma_pair_2d(dst + kWOperand + kSlabBytes, &map_dy, bar, n0 + 64, r);
           if (++stage == S) { stage = 0; phase ^= 1; }
         }
       }
       if (!ok) drain_wait();
     }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (leader && elect_one()) {
       constexpr uint32_t idesc = idesc_16bit(BF16, kWTile, kWTile) | kIdescTransA | kIdescTransB;
       int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0, tail_phase = 0;      // tail_phase: one bit per stage
+      uint32_t phase = 0, acc_phase = 0, tail_phase = 0;
+      auto block = [&](uint32_t addr, uint32_t tmem_d, bool accumulate) {
+        const uint64_t adesc = smem_desc_mn_sw128(addr), bdesc = smem_desc_mn_sw128(addr + kWOperand);
+#pragma unroll
+        for (int k = 0; k < BK / UMMA_K; ++k)
+          umma_bf16_pair(tmem_d, adesc + static_cast<uint64_t>(k * 128), bdesc + static_cast<uint64_t>(k * 128), idesc, accumulate || k != 0);
+      };
       bool ok = true;
       for (int tile = first; tile < num_tiles && ok; tile += step) {
-        const int e = tile / per_group, rows = table.row_start[e + 1] - table.row_start[e];
+        const int e = tile / per_group, rows = row_start[e + 1] - row_start[e];
         if (rows == 0) continue;
         if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1, abort_flag)) {
           gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 1, acc);
@@ -156,58 +163,66 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
         }
         tc_fence_after_sync();
         const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * kWTile);
-        for (int r = 0; r < rows; r += BK) {
+        for (int r = 0; r + BK <= rows; r += BK) {
           if (!mbar_wait(&full_bar[stage], phase, abort_flag)) {
             gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_FULL, 1, stage);
             ok = false;
             break;
           }
-          if (rows - r < BK) {
-            if (!mbar_wait(&tail_ready[stage], (tail_phase >> stage) & 1u, abort_flag)) {
-              gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_FULL, 3, stage);
-              ok = false;
-              break;
-            }
-            tail_phase ^= 1u << stage;
-          }
           tc_fence_after_sync();
-          const uint32_t addr = smem_u32(stage_base + static_cast<size_t>(stage) * kWStageBytes);
-          const uint64_t adesc = smem_desc_mn_sw128(addr), bdesc = smem_desc_mn_sw128(addr + kWOperand);
-#pragma unroll
-          for (int k = 0; k < BK / UMMA_K; ++k)
-            umma_bf16_pair(tmem_d, adesc + static_cast<uint64_t>(k * 128), bdesc + static_cast<uint64_t>(k * 128), idesc, (r | k) != 0);
+          block(smem_u32(stage_base + static_cast<size_t>(stage) * kWStageBytes), tmem_d, r != 0);
           tc_commit_pair(&empty_bar[stage], 3);
           if (++stage == S) { stage = 0; phase ^= 1; }
+        }
+        if (ok && rows % BK != 0) {
+          if (!mbar_wait(tail_ready, tail_phase, abort_flag)) {
+            gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_FULL, 1, S);
+            break;
+          }
+          tail_phase ^= 1;
+          tc_fence_after_sync();
+          block(smem_u32(tail_base), tmem_d, rows > BK);
+          tc_commit_pair(tail_empty, 3);
         }
         if (ok) tc_commit_pair(&acc_full[acc], 3);
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
     }
   } else if (warp == 2 + kWEpilogueWarps) {
-    int stage = 0;
-    uint32_t tail_phase = 0;                     // one bit per stage
+    uint32_t phase = 0;
     for (int tile = first; tile < num_tiles; tile += step) {
-      const int e = tile / per_group, rows = table.row_start[e + 1] - table.row_start[e];
-      const int blocks = (rows + BK - 1) / BK, left = rows % BK;
-      if (left != 0) {
-        const int s = (stage + blocks - 1) % S;
-        bool ok = mbar_wait(&tail_full[s], (tail_phase >> s) & 1u, abort_flag);
-        ok = __all_sync(kFullMask, ok);
-        if (!ok) {
-          if (lane == 0) gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_FULL, 3, s);
-          break;
+      int e, n0, k0;
+      locate(tile, e, n0, k0);
+      n0 += static_cast<int>(rank) * BM;
+      k0 += static_cast<int>(rank) * BM;
+      const int left = (row_start[e + 1] - row_start[e]) % BK, r0 = row_start[e + 1] - left;
+      if (left == 0) continue;
+      bool ok = mbar_wait_warp(tail_empty, phase ^ 1, abort_flag);
+      if (ok) {
+        if (elect_one()) {
+          mbar_expect_tx(tail_full, kWStageBytes);
+          tma_load_2d(tail_base, &map_x, tail_full, k0, r0);
+          tma_load_2d(tail_base + kSlabBytes, &map_x, tail_full, k0 + 64, r0);
+          tma_load_2d(tail_base + kWOperand, &map_dy, tail_full, n0, r0);
+          tma_load_2d(tail_base + kWOperand + kSlabBytes, &map_dy, tail_full, n0 + 64, r0);
         }
-        tail_phase ^= 1u << s;
-        // four slabs of 64 rows x 128 bytes: 8 lanes clear a row of each
-        uint8_t* base = stage_base + static_cast<size_t>(s) * kWStageBytes + (lane % 8) * 16;
-        for (int r = left + lane / 8; r < BK; r += 4)
-#pragma unroll
-          for (int slab = 0; slab < 4; ++slab) *reinterpret_cast<uint4*>(base + slab * kSlabBytes + r * 128) = make_uint4(0, 0, 0, 0);
-        fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tail_ready[s]), 0));
+        ok = mbar_wait_warp(tail_full, phase, abort_flag);
+        if (!ok) drain_wait();
       }
-      stage = (stage + blocks) % S;
+      if (!ok) {
+        if (lane == 0) gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_FULL, 3, 0);
+        break;
+      }
+      phase ^= 1;
+      // four slabs of 64 rows x 128 bytes: 8 lanes clear a row of each
+      for (int r = left + lane / 8; r < BK; r += 4)
+#pragma unroll
+        for (int slab = 0; slab < 4; ++slab)
+          *reinterpret_cast<uint4*>(tail_base + slab * kSlabBytes + r * 128 + (lane % 8) * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(tail_ready), 0));
     }
   } else {
     const int quarter = warp % 4;
@@ -216,10 +231,9 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
     for (int tile = first; tile < num_tiles; tile += step) {
       int e, n0, k0;
       locate(tile, e, n0, k0);
-      const bool empty = table.row_start[e + 1] == table.row_start[e];
+      const bool empty = row_start[e + 1] == row_start[e];
       if (!empty) {
-        bool ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag);
-        ok = __all_sync(kFullMask, ok);
+        bool ok = mbar_wait_warp(&acc_full[acc], acc_phase, abort_flag);
         if (!ok) {
           if (lane == 0) gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 2, acc);
           break;
