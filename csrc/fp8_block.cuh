@@ -34,32 +34,32 @@ __device__ __forceinline__ void fma2(float2& acc, float2 scale, uint32_t lo, uin
   asm("mov.b64 {%0, %1}, %2;" : "=f"(acc.x), "=f"(acc.y) : "l"(a));
 }
 
-// The scale of one row and one 128-column block of the result for every block of K, loaded two blocks ahead of its use and
-// multiplied only then: a load from L2 takes longer than a block.
+// The scales of one row and one 128-column block of the result, U blocks of K at a time: while U are used, the next U are on their way
+// from L2, and they are multiplied when their turn comes.  (One block ahead, every block took as long as a load.)
+template <int U>
 struct ScaleStream {
   const float *sa, *sb;
   long long step;
   int left;
-  float a0, b0, a1, b1;
+  float now[U], a[U], b[U];
   __device__ __forceinline__ ScaleStream(const float* sa_, long long step_, const float* sb_, int blocks, bool active)
-      : sa(sa_), sb(sb_), step(step_), left(active ? blocks : 0), a0(0.0f), b0(0.0f), a1(0.0f), b1(0.0f) {
-    fetch(a0, b0);
-    fetch(a1, b1);
+      : sa(sa_), sb(sb_), step(step_), left(active ? blocks : 0) {
+    fetch();
   }
-  __device__ __forceinline__ void fetch(float& a, float& b) {
-    if (left <= 0) return;
-    a = *sa;
-    b = *sb;
-    sa += step;
-    ++sb;
-    --left;
+  __device__ __forceinline__ void fetch() {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      a[i] = i < left ? sa[i * step] : 0.0f;
+      b[i] = i < left ? sb[i] : 0.0f;
+    }
+    sa += U * step;
+    sb += U;
+    left -= U;
   }
-  __device__ __forceinline__ float next() {
-    const float s = a0 * b0;
-    a0 = a1;
-    b0 = b1;
-    fetch(a1, b1);
-    return s;
+  __device__ __forceinline__ void advance() {      // before blocks 0, U, 2 U ..: now[0 .. U - 1] are theirs
+#pragma unroll
+    for (int i = 0; i < U; ++i) now[i] = a[i] * b[i];
+    fetch();
   }
 };
 

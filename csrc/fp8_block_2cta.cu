@@ -3,10 +3,8 @@
 //
 // Each CTA loads its own 128 rows of `a` and half of the weight rows, 32 KB per block of K where one CTA on its own would load
 // 48 KB for 128 x 256: an SM takes in about 64 bytes per clock from L2, and a block is 512 clocks of the tensor core.
-// Every block of K has accumulators of its own, one for each half of the columns (one block of weight scales), two of each; a
-// warpgroup per half adds scale * accumulator to 128 fp32 sums per thread.  An accumulator's way to the warps and back (commit, wait,
-// loads, arrival at the leader) takes longer than a block: with two accumulators of 256 columns the tensor core waited for it, now
-// it has one and a half blocks of work meanwhile.  The sums and the 64 registers in flight need
+// Every block of K has an accumulator of its own, 256 columns, two of them; eight warps (two warpgroups, a quarter of the rows and
+// half of the columns each) add scale * accumulator to 128 fp32 sums per thread.  Those sums and the 64 registers in flight need
 // more than the 168 registers that 384 threads can have, so the load and MMA warpgroup hands its registers over (setmaxnreg:
 // 40 + 232 + 232 = 3 x 168); with 168, the sums spilled, which doubled the traffic to L2.
 //
@@ -32,9 +30,7 @@ constexpr int kFPTile = 256;
 constexpr int kFPOperand = 128 * kFBlock;        // 16 KB
 constexpr int kFPStageBytes = 2 * kFPOperand;
 constexpr int kFPStages = 6;
-constexpr int kFPHalf = kFPTile / 2;
-constexpr int kFPAccs = 4;                       // half h of block kb: accumulator 2 * (kb % 2) + h
-constexpr int kFPTmemCols = kFPAccs * kFPHalf;
+constexpr int kFPTmemCols = 2 * kFPTile;
 constexpr size_t kFPSmem = 1024 + static_cast<size_t>(kFPStages) * kFPStageBytes + 256;
 constexpr int kLaunchRegs = 168, kLoadRegs = 40, kSumRegs = 232;
 static_assert(kLoadRegs + 2 * kSumRegs <= 3 * kLaunchRegs, "the warpgroups share the registers that the CTA was launched with");
@@ -56,8 +52,8 @@ fp8_block_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
   __shared__ int s_skip;
   uint8_t* stage_base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(stage_base + static_cast<size_t>(S) * kFPStageBytes);
-  uint64_t *full_bar = bars, *empty_bar = bars + S, *acc_full = bars + 2 * S, *acc_empty = bars + 2 * S + kFPAccs;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 2 * kFPAccs);
+  uint64_t *full_bar = bars, *empty_bar = bars + S, *acc_full = bars + 2 * S, *acc_empty = bars + 2 * S + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -74,9 +70,9 @@ fp8_block_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
-    for (int a = 0; a < kFPAccs; ++a) {
+    for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], kFPEpilogueWarps);      // four warps in each CTA
+      mbar_init(&acc_empty[a], 2 * kFPEpilogueWarps);
     }
     *abort_flag = 0;
     mbar_fence_init();
@@ -110,7 +106,7 @@ fp8_block_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
       for (int tile = first; tile < num_tiles && ok; tile += step) {
         int row, column;
         locate(tile, e, row, column);
-        column += static_cast<int>(rank) * 64;     // of either half, 64 columns lie in this CTA
+        column += static_cast<int>(rank) * (kFPTile / 2);
         for (int kb = 0; kb < k_blocks; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) {
             gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_EMPTY, 0, stage);
@@ -122,52 +118,47 @@ fp8_block_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
           const uint32_t bar = map_to_cta(smem_u32(&full_bar[stage]), 0);
           tma_pair_2d(a_dst, &map_a, bar, kb * kFBlock, row);
           tma_pair_3d(a_dst + kFPOperand, &map_w, bar, kb * kFBlock, column, e);
-          tma_pair_3d(a_dst + kFPOperand + kFPOperand / 2, &map_w, bar, kb * kFBlock, column + kFPHalf, e);
           if (++stage == S) { stage = 0; phase ^= 1; }
         }
       }
       if (!ok) drain_wait();
     } else if (warp == 1 && leader && elect_one()) {
-      constexpr uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(kFPHalf >> 3) << 17) | (static_cast<uint32_t>(kFPTile >> 4) << 24);
-      int stage = 0;
-      uint32_t phase = 0, block = 0;             // blocks of all tiles: accumulators and their phases follow from it
+      constexpr uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(kFPTile >> 3) << 17) | (static_cast<uint32_t>(kFPTile >> 4) << 24);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       for (int tile = first; tile < num_tiles && ok; tile += step) {
-        for (int kb = 0; kb < k_blocks && ok; ++kb, ++block) {
-          if (!mbar_wait_soon(&full_bar[stage], phase, abort_flag)) {
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1, abort_flag)) {
+            gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 1, acc);
+            ok = false;
+            break;
+          }
+          if (!mbar_wait(&full_bar[stage], phase, abort_flag)) {
             gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_FULL, 1, stage);
             ok = false;
             break;
           }
+          tc_fence_after_sync();
           const uint32_t a_addr = smem_u32(stage_base + static_cast<size_t>(stage) * kFPStageBytes);
           const uint64_t adesc = smem_desc_sw128(a_addr), bdesc = smem_desc_sw128(a_addr + kFPOperand);
-          const uint32_t pair = (block & 1u) * 2u, acc_phase = (block >> 1) & 1u;
+          const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * kFPTile);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (!mbar_wait_soon(&acc_empty[pair + h], acc_phase ^ 1u, abort_flag)) {
-              gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 1, pair + h);
-              ok = false;
-              break;
-            }
-            tc_fence_after_sync();
-            const uint32_t tmem_d = tmem_base + (pair + h) * kFPHalf;
-#pragma unroll
-            for (int k = 0; k < kFBlock / 32; ++k)
-              umma_f8_pair(tmem_d, adesc + static_cast<uint64_t>(k * 2), bdesc + static_cast<uint64_t>(h * (kFPOperand / 2 / 16) + k * 2), idesc, k != 0);
-            tc_commit_pair(&acc_full[pair + h], 3);
-          }
+          for (int k = 0; k < kFBlock / 32; ++k)
+            umma_f8_pair(tmem_d, adesc + static_cast<uint64_t>(k * 2), bdesc + static_cast<uint64_t>(k * 2), idesc, k != 0);
           tc_commit_pair(&empty_bar[stage], 3);
+          tc_commit_pair(&acc_full[acc], 3);
           if (++stage == S) { stage = 0; phase ^= 1; }
+          if (++acc == 2) { acc = 0; acc_phase ^= 1; }
         }
       }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
     const int quarter = warp % 4, half = (warp - 4) / 4;
-    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint32_t leader_empty = map_to_cta(smem_u32(&acc_empty[half]), 0);
-    int e = 0;
-    uint32_t block = 0;
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(half * COLS);
+    int acc = 0, e = 0;
+    uint32_t acc_phase = 0;
     bool ok = true;
     for (int tile = first; tile < num_tiles && ok; tile += step) {
       int row, column;
@@ -178,18 +169,22 @@ fp8_block_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
       float2 sum[COLS / 2];
 #pragma unroll
       for (int i = 0; i < COLS / 2; ++i) sum[i] = make_float2(0.0f, 0.0f);
-      ScaleStream scales(g.sa + min(row, g.rows - 1) * g.sa_row, g.sa_block, weight_scales(g, e, column, k_blocks), k_blocks, left > 0);
-      for (int kb = 0; kb < k_blocks; ++kb, ++block) {
-        const float scale = scales.next();
-        const uint32_t acc = (block & 1u) * 2u + half;
-        ok = mbar_wait_warp(&acc_full[acc], (block >> 1) & 1u, abort_flag);
+      ScaleStream<4> scales(g.sa + min(row, g.rows - 1) * g.sa_row, g.sa_block, weight_scales(g, e, column, k_blocks), k_blocks, left > 0);
+      for (int kb0 = 0; kb0 < k_blocks && ok; kb0 += 4) {
+       scales.advance();
+#pragma unroll
+       for (int j = 0; j < 4; ++j) {
+        if (kb0 + j >= k_blocks) break;
+        const float scale = scales.now[j];
+        ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag);
+        ok = __all_sync(kFullMask, ok);
         if (!ok) {
           if (lane == 0) gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 2, acc);
           break;
         }
         tc_fence_after_sync();
         const float2 s2 = make_float2(scale, scale);
-        const uint32_t taddr = lane_base + acc * kFPHalf;
+        const uint32_t taddr = lane_base + static_cast<uint32_t>(acc * kFPTile);
         uint32_t r0[32], r1[32];                 // the next 32 columns are on their way while these are added
         if (left > 0) {
           tmem_ld32(taddr, r0);
@@ -209,11 +204,13 @@ fp8_block_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_relaxed(leader_empty + (block & 1u) * 16u);
+        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&acc_empty[acc]), 0));
         if (left > 0) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) fma2(sum[48 + i], s2, r1[2 * i], r1[2 * i + 1]);
         }
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+       }
       }
       if (ok && lane < left) store_row(g, row, column, sum);
     }

@@ -36,15 +36,18 @@ constexpr int kFThreads = 320;                   // 0 producer, 1 MMA, 2..9 scal
 constexpr int kFEpilogueWarps = 8;
 constexpr int kFSmemLimit = 216 * 1024;
 
+// U blocks of K share a stage, an accumulator and every wait: an exchange between the roles costs some hundred clocks whatever it
+// hands over, a block of 32 columns is 64 clocks of the tensor core.
 template <int BN, int AR> struct FGeometry {
+  static constexpr int kU = AR == 32 && BN <= 64 ? 4 : 2;
   static constexpr int kABytes = AR * kFBlock;
   static constexpr int kBBytes = BN * kFBlock;
-  static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kBehind = (BM - AR) * kFBlock;       // what the MMA reads behind the rows of the last stage
+  static constexpr int kStageBytes = kU * (kABytes + kBBytes);        // kU blocks of a, then kU blocks of w
+  static constexpr int kBehind = (BM - AR) * kFBlock;       // what the MMA may read behind the last stage
   static constexpr int kFit = (kFSmemLimit - kBehind) / kStageBytes;
-  static constexpr int kStages = kFit < 16 ? kFit : 16;
-  static constexpr int kAccs = 512 / BN < 4 ? 512 / BN : 4;
-  static constexpr int kTmemCols = kAccs * BN;
+  static constexpr int kStages = kFit < 8 ? kFit : 8;
+  static constexpr int kAccs = 512 / (kU * BN) < 4 ? 512 / (kU * BN) : 4;
+  static constexpr int kTmemCols = kAccs * kU * BN;
   static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStageBytes + kBehind + 512;
 };
 
@@ -64,11 +67,21 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void load_part(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+__device__ __forceinline__ void load_part(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
+__device__ __forceinline__ void wait_part(uint32_t (&r)[32]) { wait_loaded(r); }
+__device__ __forceinline__ void wait_part(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :: "memory");
+}
+
 template <int BN, int AR>
 __global__ void __launch_bounds__(kFThreads, 1)
 fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const FArgs g) {
   using Geo = FGeometry<BN, AR>;
-  constexpr int S = Geo::kStages, ACCS = Geo::kAccs;
+  constexpr int S = Geo::kStages, ACCS = Geo::kAccs, U = Geo::kU;
   constexpr int COLS = BN / 2;                   // columns of one epilogue thread
   constexpr int CHUNK = COLS < 32 ? COLS : 32;
   static_assert(CHUNK == 32 || CHUNK == 16, "");
@@ -126,16 +139,21 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
         int row, column;
         locate(tile, e, row, column);
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        for (int kb = 0; kb < k_blocks; kb += U) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) {
             gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_EMPTY, 0, stage);
             ok = false;
             break;
           }
-          uint8_t* a_dst = stage_base + static_cast<size_t>(stage) * Geo::kStageBytes;
-          mbar_expect_tx(&full_bar[stage], Geo::kStageBytes);
-          tma_load_2d(a_dst, &map_a, &full_bar[stage], kb * kFBlock, row);
-          tma_load_3d(a_dst + Geo::kABytes, &map_w, &full_bar[stage], kb * kFBlock, column, e);
+          uint8_t* dst = stage_base + static_cast<size_t>(stage) * Geo::kStageBytes;
+          const int here = min(U, k_blocks - kb);
+          mbar_expect_tx(&full_bar[stage], here * (Geo::kABytes + Geo::kBBytes));
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            if (u >= here) break;
+            tma_load_2d(dst + u * Geo::kABytes, &map_a, &full_bar[stage], (kb + u) * kFBlock, row);
+            tma_load_3d(dst + U * Geo::kABytes + u * Geo::kBBytes, &map_w, &full_bar[stage], (kb + u) * kFBlock, column, e);
+          }
           if (++stage == S) { stage = 0; phase ^= 1; }
         }
       }
@@ -148,7 +166,7 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        for (int kb = 0; kb < k_blocks; kb += U) {
           if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1, abort_flag)) {
             gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 1, acc);
             ok = false;
@@ -161,11 +179,17 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           }
           tc_fence_after_sync();
           const uint32_t a_addr = smem_u32(stage_base + static_cast<size_t>(stage) * Geo::kStageBytes);
-          const uint64_t adesc = smem_desc_sw128(a_addr), bdesc = smem_desc_sw128(a_addr + Geo::kABytes);
-          const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * BN);
+          const uint64_t adesc = smem_desc_sw128(a_addr), bdesc = smem_desc_sw128(a_addr + U * Geo::kABytes);
+          const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * U * BN);
+          const int here = min(U, k_blocks - kb);
 #pragma unroll
-          for (int k = 0; k < kFBlock / 32; ++k)
-            umma_f8(tmem_d, adesc + static_cast<uint64_t>(k * 2), bdesc + static_cast<uint64_t>(k * 2), idesc, k != 0);
+          for (int u = 0; u < U; ++u) {
+            if (u >= here) break;
+#pragma unroll
+            for (int k = 0; k < kFBlock / 32; ++k)
+              umma_f8(tmem_d + u * BN, adesc + static_cast<uint64_t>(u * (Geo::kABytes / 16) + k * 2),
+                      bdesc + static_cast<uint64_t>(u * (Geo::kBBytes / 16) + k * 2), idesc, k != 0);
+          }
           tc_commit(&empty_bar[stage]);
           tc_commit(&acc_full[acc]);
           if (++stage == S) { stage = 0; phase ^= 1; }
@@ -187,34 +211,33 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       float2 sum[COLS / 2];
 #pragma unroll
       for (int i = 0; i < COLS / 2; ++i) sum[i] = make_float2(0.0f, 0.0f);
-      ScaleStream scales(g.sa + min(row, g.rows - 1) * g.sa_row, g.sa_block, weight_scales(g, e, column, k_blocks), k_blocks, left > 0);
-      for (int kb = 0; kb < k_blocks; ++kb) {
-        const float scale = scales.next();
-        ok = mbar_wait_warp(&acc_full[acc], acc_phase, abort_flag);
+      ScaleStream<U> scales(g.sa + min(row, g.rows - 1) * g.sa_row, g.sa_block, weight_scales(g, e, column, k_blocks), k_blocks, left > 0);
+      for (int kb = 0; kb < k_blocks; kb += U) {
+        scales.advance();
+        ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag);
+        ok = __all_sync(kFullMask, ok);
         if (!ok) {
           if (lane == 0) gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 2, acc);
           break;
         }
         tc_fence_after_sync();
+        const int here = min(U, k_blocks - kb);
+        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * U * BN + half * COLS);
         if (left > 0) {
-          const float2 s2 = make_float2(scale, scale);
-          const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BN + half * COLS);
+          // PART columns of a block at a time; the next ones are on their way while these are added
+          constexpr int PARTS = U * COLS / CHUNK, PER = COLS / CHUNK;
+          uint32_t r[2][CHUNK];
+          load_part(taddr, r[0]);
 #pragma unroll
-          for (int c = 0; c < COLS; c += CHUNK) {
-            if constexpr (CHUNK == 32) {
-              uint32_t r[32];
-              tmem_ld32(taddr + c, r);
-              wait_loaded(r);
+          for (int q = 0; q < PARTS; ++q) {
+            if (q / PER >= here) break;
+            wait_part(r[q % 2]);
+            if (q + 1 < PARTS) load_part(taddr + (q + 1) / PER * BN + (q + 1) % PER * CHUNK, r[(q + 1) % 2]);
+            const float2 s2 = make_float2(scales.now[q / PER], scales.now[q / PER]);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) fma2(sum[c / 2 + i], s2, r[2 * i], r[2 * i + 1]);
-            } else {
-              uint32_t r[16];
-              tmem_ld16(taddr + c, r);
-              tc_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 8; ++i) fma2(sum[c / 2 + i], s2, r[2 * i], r[2 * i + 1]);
-            }
+            for (int i = 0; i < CHUNK / 2; ++i) fma2(sum[q % PER * (CHUNK / 2) + i], s2, r[q % 2][2 * i], r[q % 2][2 * i + 1]);
           }
+          tc_wait_ld();
         }
         tc_fence_before_sync();
         __syncwarp();
@@ -282,7 +305,7 @@ cudaError_t launch_fp8_block_gemm(const void* a, long long lda, const float* sa,
   const CUtensorMap map_a = make_swizzled_map(a, 1, 2, a_dims, a_strides, a_box);
   const uint64_t w_dims[3] = {static_cast<uint64_t>(k), static_cast<uint64_t>(n), static_cast<uint64_t>(groups)};
   const uint64_t w_strides[2] = {static_cast<uint64_t>(ldw), static_cast<uint64_t>(lde)};
-  const uint32_t w_box[3] = {kFBlock, static_cast<uint32_t>(bn == 256 ? 64 : bn), 1};
+  const uint32_t w_box[3] = {kFBlock, static_cast<uint32_t>(bn == 256 ? 128 : bn), 1};
   const CUtensorMap map_w = make_swizzled_map(w, 1, 3, w_dims, w_strides, w_box);
   const int tile_rows = bn == 256 ? 2 * BM : BM;
   const long long active = groups < rows ? groups : rows, most = static_cast<long long>((n + bn - 1) / bn) * (rows / tile_rows + active);
