@@ -5,16 +5,19 @@
 // a, w: e4m3; sa: one scale per row and 128 values; sb: one per 128 x 128 values; d: bf16.
 //
 // The scales are arbitrary fp32 numbers, so the tensor core cannot apply them (its block scales are powers of two): every block of
-// K gets an accumulator of its own in tensor memory (tcgen05.mma kind::f8f6f4, four instructions of K = 32), and eight warps add
-// scale * accumulator to fp32 sums in registers while the tensor core fills the next accumulator.  The lane of an accumulator is
-// a row, so that one number per thread and block scales all of its columns.  Tiles are 128 rows x BN columns of one CTA: warps
-// 2 .. 9 take a quarter of the rows and half of the columns each.
+// K gets columns of its own in tensor memory (tcgen05.mma kind::f8f6f4, four instructions of K = 32), and eight warps add scale *
+// accumulator to fp32 sums in registers while the tensor core goes on.  The lane of an accumulator is a row, so that one number per
+// thread and block scales all of its columns.  Tiles are 128 rows x BN columns of one CTA: warps 2 .. 9 take a quarter of the rows
+// and half of the columns each.
 //
-// The operands of a 128 x 256 tile would take more of L2 than an SM gets (48 KB per block of K), so large products run on CTA pairs
-// (fp8_block_2cta.cu); this kernel has the tiles of up to 128 columns that small ones need to fill the GPU.
+// What bounds it: an exchange between the roles (commit, wait, arrival) costs some hundred clocks whatever it hands over, so two or
+// four blocks of K share one (8192 x 4096 x 14336: 625 us with one, 448 with two); the operands of a 128 x 128 tile come from L2 at 19
+// TB/s, which alone takes 405 us there.  Tried: 128 x 256 tiles (128 sums a thread spill, and a spilled value comes back from L2:
+// 614 us), CTA pairs with 256 x 256 (481: one block per accumulator) and 256 x 128 tiles (438, and 549 against 519 us at 8192 x 14336 x
+// 4096).
 //
-// With at most 32 rows in every tile only 32 rows of `a` are loaded; the tensor core then reads whatever follows in shared memory
-// as the other rows (still inside the allocation) and their results are not read.
+// With at most 32 rows in all only 32 rows of `a` are loaded; the tensor core then reads whatever follows in shared memory as
+// the other rows (still inside the allocation) and their results are not read.
 //
 // Every wait is bounded (gemm_sm100.cuh).
 #include <cuda.h>
@@ -24,13 +27,129 @@
 #include "expert_ops.h"
 #include "gemm_sm100.cuh"
 #include "gemm_sm100.h"
-#include "fp8_block.cuh"
 #include "grouped_common.cuh"
 
 namespace msccl {
 namespace sm100 {
 
 namespace {
+
+constexpr int kFBlock = 128;                     // K values per scale = bytes per shared-memory row
+constexpr int kFGroupTileRows = 2048;            // rows that a group of tiles walks together (L2, see tile_coords)
+
+struct FArgs {
+  const int* offsets;                            // nullptr: one group of all rows
+  const float *sa, *sb;
+  long long sa_row, sa_block;                    // strides of sa
+  __nv_bfloat16* out;
+  long long ldo;
+  int rows, groups, n, k;
+  int zero_rest;
+  int* error_words;
+};
+
+// Two fp32 sums at once: acc += scale * v.
+__device__ __forceinline__ void fma2(float2& acc, float2 scale, uint32_t lo, uint32_t hi) {
+  unsigned long long a, s, v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(acc.x), "f"(acc.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(s) : "f"(scale.x), "f"(scale.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(s), "l"(v));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(acc.x), "=f"(acc.y) : "l"(a));
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void load_part(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+__device__ __forceinline__ void load_part(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
+__device__ __forceinline__ void wait_part(uint32_t (&r)[32]) { wait_loaded(r); }
+__device__ __forceinline__ void wait_part(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :: "memory");
+}
+
+// The scales of one row and one 128-column block of the result, U blocks of K at a time: while U are used, the next U are on their way
+// from L2, and they are multiplied when their turn comes.  (One block ahead, every block took as long as a load.)
+template <int U>
+struct ScaleStream {
+  const float *sa, *sb;
+  long long step;
+  int left;
+  float now[U], a[U], b[U];
+  __device__ __forceinline__ ScaleStream(const float* sa_, long long step_, const float* sb_, int blocks, bool active)
+      : sa(sa_), sb(sb_), step(step_), left(active ? blocks : 0) {
+    fetch();
+  }
+  __device__ __forceinline__ void fetch() {
+    if (left >= U) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        a[i] = *sa;
+        b[i] = sb[i];
+        sa += step;
+      }
+      sb += U;
+    } else {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        a[i] = i < left ? *sa : 0.0f;
+        b[i] = i < left ? sb[i] : 0.0f;
+        if (i + 1 < left) sa += step;
+      }
+    }
+    left -= U;
+  }
+  __device__ __forceinline__ void advance() {      // before blocks 0, U, 2 U ..: now[0 .. U - 1] are theirs
+#pragma unroll
+    for (int i = 0; i < U; ++i) now[i] = a[i] * b[i];
+    fetch();
+  }
+};
+
+// Where the scales of column block `column / 128` of group e start.
+__device__ __forceinline__ const float* weight_scales(const FArgs& g, int e, int column, int k_blocks) {
+  const int n_blocks = (g.n + kFBlock - 1) / kFBlock;
+  return g.sb + (static_cast<long long>(e) * n_blocks + min(column / kFBlock, n_blocks - 1)) * k_blocks;
+}
+
+template <typename TilesOf>
+__device__ __forceinline__ void build_table(GroupTable& table, const FArgs& g, TilesOf tiles_of) {       // whole warp
+  if (g.offsets != nullptr) {
+    build_groups(table, g.offsets, g.groups, g.rows, tiles_of);
+  } else if (threadIdx.x % 32 == 0) {
+    table.row_start[0] = table.tile_start[0] = 0;
+    table.row_start[1] = g.rows;
+    table.tile_start[1] = tiles_of(g.rows);
+  }
+}
+
+// Rows before the first group and behind the last one become zero; `warp` of `warps` all over the grid.
+__device__ __forceinline__ void zero_rest_rows(const GroupTable& table, const FArgs& g, int warp, int warps) {
+  const int head = table.row_start[0], tail = table.row_start[g.groups], rest = head + g.rows - tail, lane = threadIdx.x % 32;
+  for (int i = warp; i < rest; i += warps) {
+    uint4* dst = reinterpret_cast<uint4*>(g.out + static_cast<long long>(i < head ? i : tail + i - head) * g.ldo);
+    for (int v = lane; v < g.n / 8; v += 32) dst[v] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// One row's columns [column, column + 2 * PAIRS) as bf16, as far as the result has them (multiples of 8).
+template <int PAIRS>
+__device__ __forceinline__ void store_row(const FArgs& g, long long row, int column, const float2 (&sum)[PAIRS]) {
+  __nv_bfloat16* out = g.out + row * g.ldo + column;
+#pragma unroll
+  for (int c = 0; c < PAIRS; c += 4)
+    if (column + 2 * c < g.n)
+      *reinterpret_cast<uint4*>(out + 2 * c) = make_uint4(pack_bf16(sum[c].x, sum[c].y), pack_bf16(sum[c + 1].x, sum[c + 1].y),
+                                                          pack_bf16(sum[c + 2].x, sum[c + 2].y), pack_bf16(sum[c + 3].x, sum[c + 3].y));
+}
 
 constexpr int kFThreads = 320;                   // 0 producer, 1 MMA, 2..9 scaling and epilogue
 constexpr int kFEpilogueWarps = 8;
@@ -59,32 +178,13 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_
       ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void load_part(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
-__device__ __forceinline__ void load_part(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
-__device__ __forceinline__ void wait_part(uint32_t (&r)[32]) { wait_loaded(r); }
-__device__ __forceinline__ void wait_part(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :: "memory");
-}
-
 template <int BN, int AR>
 __global__ void __launch_bounds__(kFThreads, 1)
 fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const FArgs g) {
   using Geo = FGeometry<BN, AR>;
   constexpr int S = Geo::kStages, ACCS = Geo::kAccs, U = Geo::kU;
   constexpr int COLS = BN / 2;                   // columns of one epilogue thread
-  constexpr int CHUNK = COLS < 32 ? COLS : 32;
-  static_assert(CHUNK == 32 || CHUNK == 16, "");
+  constexpr int CHUNK = 16;
   extern __shared__ uint8_t smem_raw[];
   __shared__ GroupTable table;
   uint8_t* stage_base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -211,9 +311,13 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       float2 sum[COLS / 2];
 #pragma unroll
       for (int i = 0; i < COLS / 2; ++i) sum[i] = make_float2(0.0f, 0.0f);
-      ScaleStream<U> scales(g.sa + min(row, g.rows - 1) * g.sa_row, g.sa_block, weight_scales(g, e, column, k_blocks), k_blocks, left > 0);
-      for (int kb = 0; kb < k_blocks; kb += U) {
+      ScaleStream<2 * U> scales(g.sa + min(row, g.rows - 1) * g.sa_row, g.sa_block, weight_scales(g, e, column, k_blocks), k_blocks, left > 0);
+      for (int kb0 = 0; kb0 < k_blocks && ok; kb0 += 2 * U) {
         scales.advance();
+#pragma unroll
+        for (int turn = 0; turn < 2; ++turn) {
+        const int kb = kb0 + turn * U;
+        if (kb >= k_blocks) break;
         ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag);
         ok = __all_sync(kFullMask, ok);
         if (!ok) {
@@ -223,26 +327,34 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         tc_fence_after_sync();
         const int here = min(U, k_blocks - kb);
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * U * BN + half * COLS);
+        auto release = [&] {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[acc]);
+        };
         if (left > 0) {
-          // PART columns of a block at a time; the next ones are on their way while these are added
-          constexpr int PARTS = U * COLS / CHUNK, PER = COLS / CHUNK;
+          // CHUNK columns of a block at a time; the next ones are on their way while these are added, and the accumulator is free
+          // again before the last ones are
+          constexpr int PER = COLS / CHUNK;
           uint32_t r[2][CHUNK];
           load_part(taddr, r[0]);
 #pragma unroll
-          for (int q = 0; q < PARTS; ++q) {
+          for (int q = 0; q < U * PER; ++q) {
             if (q / PER >= here) break;
             wait_part(r[q % 2]);
-            if (q + 1 < PARTS) load_part(taddr + (q + 1) / PER * BN + (q + 1) % PER * CHUNK, r[(q + 1) % 2]);
-            const float2 s2 = make_float2(scales.now[q / PER], scales.now[q / PER]);
+            if ((q + 1) % PER != 0 || (q + 1) / PER < here)
+              load_part(taddr + (q + 1) / PER * BN + (q + 1) % PER * CHUNK, r[(q + 1) % 2]);
+            else
+              release();
+            const float2 s2 = make_float2(scales.now[turn * U + q / PER], scales.now[turn * U + q / PER]);
 #pragma unroll
             for (int i = 0; i < CHUNK / 2; ++i) fma2(sum[q % PER * (CHUNK / 2) + i], s2, r[q % 2][2 * i], r[q % 2][2 * i + 1]);
           }
-          tc_wait_ld();
+        } else {
+          release();
         }
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[acc]);
         if (++acc == ACCS) { acc = 0; acc_phase ^= 1; }
+        }
       }
       if (ok && lane < left) store_row(g, row, column, sum);
     }
@@ -278,7 +390,7 @@ cudaError_t launch(const CUtensorMap& map_a, const CUtensorMap& map_w, const FAr
 
 // a: [rows, k] e4m3 (pitch lda bytes), sa: [rows, ceil(k / 128)] with the strides given; w: [groups, n, k] e4m3 (pitch ldw, matrix
 // stride lde), sb: [groups, ceil(n / 128), ceil(k / 128)] contiguous; out: [rows, n] bf16.  k % 16 == 0, n % 8 == 0.
-// bn: 32, 64 or 128 (columns per tile of one CTA), or 256: the CTA-pair kernel; few_rows: no group has more than 32 rows.
+// bn: 32, 64 or 128 columns per tile; few_rows: there are at most 32 rows.
 cudaError_t launch_fp8_block_gemm(const void* a, long long lda, const float* sa, long long sa_row, long long sa_block, const void* w,
                                   long long ldw, long long lde, const float* sb, const int* offsets, void* out, long long ldo, int rows,
                                   int groups, int n, int k, int bn, bool few_rows, bool zero_rest, int* error_words, cudaStream_t stream) {
@@ -300,22 +412,19 @@ cudaError_t launch_fp8_block_gemm(const void* a, long long lda, const float* sa,
   g.zero_rest = zero_rest ? 1 : 0;
   g.error_words = error_words;
   const uint64_t a_dims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(rows)}, a_strides[1] = {static_cast<uint64_t>(lda)};
-  if (bn == 256) few_rows = false;
   const uint32_t a_box[2] = {kFBlock, few_rows ? 32u : static_cast<uint32_t>(BM)};
   const CUtensorMap map_a = make_swizzled_map(a, 1, 2, a_dims, a_strides, a_box);
   const uint64_t w_dims[3] = {static_cast<uint64_t>(k), static_cast<uint64_t>(n), static_cast<uint64_t>(groups)};
   const uint64_t w_strides[2] = {static_cast<uint64_t>(ldw), static_cast<uint64_t>(lde)};
-  const uint32_t w_box[3] = {kFBlock, static_cast<uint32_t>(bn == 256 ? 128 : bn), 1};
+  const uint32_t w_box[3] = {kFBlock, static_cast<uint32_t>(bn), 1};
   const CUtensorMap map_w = make_swizzled_map(w, 1, 3, w_dims, w_strides, w_box);
-  const int tile_rows = bn == 256 ? 2 * BM : BM;
-  const long long active = groups < rows ? groups : rows, most = static_cast<long long>((n + bn - 1) / bn) * (rows / tile_rows + active);
+  const long long active = groups < rows ? groups : rows, most = static_cast<long long>((n + bn - 1) / bn) * (rows / BM + active);
   if (most > (1ll << 30)) return cudaErrorInvalidValue;
   const int tiles = static_cast<int>(most);
   switch (bn) {
     case 32: return few_rows ? launch<32, 32>(map_a, map_w, g, tiles, stream) : launch<32, BM>(map_a, map_w, g, tiles, stream);
     case 64: return few_rows ? launch<64, 32>(map_a, map_w, g, tiles, stream) : launch<64, BM>(map_a, map_w, g, tiles, stream);
     case 128: return few_rows ? launch<128, 32>(map_a, map_w, g, tiles, stream) : launch<128, BM>(map_a, map_w, g, tiles, stream);
-    case 256: return launch_fp8_block_pairs(map_a, map_w, g, tiles, stream);
     default: return cudaErrorInvalidValue;
   }
 }

@@ -7,8 +7,8 @@
 // the device only: every CTA derives the same list of tiles from the offsets, so nothing is copied to the host.
 //
 // The weights are the M operand and the rows of the group the N operand of the MMA: 256 features (of a CTA pair, cta_group::2)
-// by BN rows.  The last tile of a group is then padded to a multiple of BN = 32 .. 256 rows instead of 256, and a decode batch
-// streams the weights through tiles of 32 rows.  Rows of a tile that belong to the next group only reach columns of the accumulator
+// by BN rows.  The last tile of a group is then padded to a multiple of BN = 64 .. 256 rows instead of 256, and a decode batch
+// streams the weights through tiles of 64 rows.  Rows of a tile that belong to the next group only reach columns of the accumulator
 // that are not stored, whatever they hold.  What is left of both operands behind the reduction dimension reads as zero.
 //
 // The accumulator holds a feature per lane and a row per column; the epilogue transposes it (transpose_chunk).
@@ -258,7 +258,7 @@ cudaError_t launch_by_type(bool mn_major, bool bf16, const CUtensorMap& map_w, c
 }  // namespace
 
 // w: [groups, n, k] (pitch ldw, matrix stride lde, elements); x: [rows, k] and out: [rows, n], or with `backward` x: [rows, n]
-// (dy) and out: [rows, k].  n % 8 == 0, k % 8 == 0, everything 16-byte aligned.  bn: 32, 64, 128 or 256 rows per tile.
+// (dy) and out: [rows, k].  n % 8 == 0, k % 8 == 0, everything 16-byte aligned.  bn: 64, 128 or 256 rows per tile.
 cudaError_t launch_grouped_gemm(const void* x, long long ldx, const void* w, long long ldw, long long lde, const int* offsets, void* out,
                                 long long ldo, int rows, int groups, int n, int k, bool backward, int elem, int bn, bool zero_rest,
                                 int* error_words, cudaStream_t stream) {
@@ -290,7 +290,6 @@ cudaError_t launch_grouped_gemm(const void* x, long long ldx, const void* w, lon
   const int most_tiles = most < 1 ? 1 : static_cast<int>(most);
   const bool bf16 = elem == kElemBF16;
   switch (bn) {
-    case 32: return launch_by_type<32>(backward, bf16, map_w, map_x, g, most_tiles, stream);
     case 64: return launch_by_type<64>(backward, bf16, map_w, map_x, g, most_tiles, stream);
     case 128: return launch_by_type<128>(backward, bf16, map_w, map_x, g, most_tiles, stream);
     case 256: return launch_by_type<256>(backward, bf16, map_w, map_x, g, most_tiles, stream);

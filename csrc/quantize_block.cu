@@ -6,7 +6,7 @@
 // definition alone.  Infinite values make the scale infinite (the block becomes NaN and zeros), NaN makes the whole block NaN:
 // neither can vanish.  The floor keeps the scale of a block of zeros, or of values below 2^-100, a normal number.
 //
-// Memory bound: a row's 128 bf16 values are 16 lanes x 16 bytes in, 16 lanes x 8 bytes out.
+// Memory bound (5 TB/s): a row's 128 bf16 values are 16 lanes x 16 bytes in, 16 lanes x 8 bytes out.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -63,60 +63,46 @@ __device__ __forceinline__ float block_scale(uint32_t bits) {
 // "Computation of elementary functions on the IBM RISC System/6000 processor", 1990, theorem on division).  Scales are between
 // 2^-109 and 2^120, so neither the reciprocal nor a remainder that matters leaves the range of exact numbers; an infinite or NaN scale
 // takes the division itself.  Eight divisions per thread made the kernel slower than memory (8192 x 14336: 123 us).
-struct Divider {
-  float scale, reciprocal;
-  bool plain;
-  __device__ __forceinline__ float operator()(float x) const {
-    if (plain) return __fdiv_rn(x, scale);
-    const float q = x * reciprocal;
-    return fmaf(fmaf(-q, scale, x), reciprocal, q);
-  }
-};
-__device__ __forceinline__ Divider divider(float scale) {
-  Divider d;
-  d.scale = scale;
-  d.reciprocal = __frcp_rn(scale);
-  d.plain = !(scale < INFINITY);
-  return d;
-}
-__device__ __forceinline__ uint2 quantize8(const float (&v)[8], const Divider& divide) {
+__device__ __forceinline__ uint2 to_e4m3(const float (&v)[8]) {
   uint32_t p[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    p[i] = __nv_cvt_float2_to_fp8x2(make_float2(divide(v[2 * i]), divide(v[2 * i + 1])), __NV_SATFINITE, __NV_E4M3);
+  for (int i = 0; i < 4; ++i) p[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
   return make_uint2(p[0] | p[1] << 16, p[2] | p[3] << 16);
 }
+__device__ __forceinline__ uint2 quantize8(const float (&v)[8], float scale) {
+  float q[8];
+  if (scale < INFINITY) {
+    const float reciprocal = __frcp_rn(scale);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      q[i] = v[i] * reciprocal;
+      q[i] = fmaf(fmaf(-q[i], scale, v[i]), reciprocal, q[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = __fdiv_rn(v[i], scale);
+  }
+  return to_e4m3(q);
+}
 
-// 16 lanes take one block of R consecutive rows.
-template <typename T, int R>
+// 16 lanes take one block of one row; threadIdx.x runs along the row (whole blocks), threadIdx.y over rows.  (Blocks numbered through, a
+// division of 64-bit numbers per thread, took 123 us for 8192 x 14336 instead of 92; several rows per thread gain nothing.)
+template <typename T>
 __global__ void __launch_bounds__(kQThreads)
 quantize_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q, float* __restrict__ scales, int rows, int k,
                      long long s_row, long long s_block) {
-  const int blocks = (k + 127) / 128;
-  const long long item = (static_cast<long long>(blockIdx.x) * kQThreads + threadIdx.x) / 16;
-  const long long row = item / blocks * R;
-  if (row >= rows) return;                                          // uniform for those 16 lanes
-  const int b = static_cast<int>(item % blocks), col = b * 128 + static_cast<int>(threadIdx.x % 16) * 8;
-  const unsigned int mask = 0xffffu << (threadIdx.x & 16);
-  float v[R][8];
+  const long long row = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
+  const int col = (blockIdx.y * blockDim.x + threadIdx.x) * 8, b = col / 128;
+  if (row >= rows || b * 128 >= k) return;                          // uniform for those 16 lanes
+  const unsigned int mask = 0xffffu << ((threadIdx.y * blockDim.x + threadIdx.x) & 16);
+  float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  if (col < k) load8(x + row * ldx + col, v);
+  uint32_t m = largest_bits(v);
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    if (row + i < rows && col < k) load8(x + (row + i) * ldx + col, v[i]);
-    else
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-  }
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    uint32_t m = largest_bits(v[i]);
-#pragma unroll
-    for (int off = 8; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(mask, m, off));
-    const Divider divide = divider(block_scale(m));
-    if (row + i < rows) {
-      if (col < k) *reinterpret_cast<uint2*>(q + (row + i) * k + col) = quantize8(v[i], divide);
-      if (threadIdx.x % 16 == 0) scales[(row + i) * s_row + b * s_block] = divide.scale;
-    }
-  }
+  for (int off = 8; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(mask, m, off));
+  const float scale = block_scale(m);
+  if (col < k) *reinterpret_cast<uint2*>(q + row * k + col) = quantize8(v, scale);
+  if (threadIdx.x % 16 == 0) scales[row * s_row + b * s_block] = scale;
 }
 
 template <typename T>
@@ -142,13 +128,13 @@ quantize_blocks_kernel(const T* __restrict__ w, long long ldw, long long lde, ui
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kQThreads / 32; ++i) m = max(m, part[i]);
-  const Divider divide = divider(block_scale(m));
+  const float scale = block_scale(m);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int row = row0 + 16 * i;
-    if (row < n && col < k) *reinterpret_cast<uint2*>(q + (static_cast<long long>(e) * n + row) * k + col) = quantize8(v[i], divide);
+    if (row < n && col < k) *reinterpret_cast<uint2*>(q + (static_cast<long long>(e) * n + row) * k + col) = quantize8(v[i], scale);
   }
-  if (threadIdx.x == 0) scales[(static_cast<long long>(e) * gridDim.y + nb) * gridDim.x + kb] = divide.scale;
+  if (threadIdx.x == 0) scales[(static_cast<long long>(e) * gridDim.y + nb) * gridDim.x + kb] = scale;
 }
 
 }  // namespace
@@ -166,18 +152,12 @@ quantize_blocks_kernel(const T* __restrict__ w, long long ldw, long long lde, ui
 cudaError_t launch_quantize_rows(const void* x, long long ldx, void* q, float* scales, long long s_row, long long s_block, int rows, int k,
                                  int elem, cudaStream_t stream) {
   if (rows < 1 || k < 16 || k % 16 != 0) return cudaErrorInvalidValue;
-  // four rows a thread where that still fills the GPU: more loads in flight
-  const long long blocks = (k + 127) / 128;
-  const int step = rows * blocks >= 1 << 16 ? 4 : 1;
-  const long long grid = (rows + step - 1) / step * blocks / (kQThreads / 16) + 1;
-  if (grid > 0x7fffffffll) return cudaErrorInvalidValue;
-  if (step == 4) {
-    MSCCL_BY_ELEM(elem, (quantize_rows_kernel<T, 4><<<static_cast<int>(grid), kQThreads, 0, stream>>>(
-                            static_cast<const T*>(x), ldx, static_cast<uint8_t*>(q), scales, rows, k, s_row, s_block)));
-  } else {
-    MSCCL_BY_ELEM(elem, (quantize_rows_kernel<T, 1><<<static_cast<int>(grid), kQThreads, 0, stream>>>(
-                            static_cast<const T*>(x), ldx, static_cast<uint8_t*>(q), scales, rows, k, s_row, s_block)));
-  }
+  const int blocks = (k + 127) / 128, across = blocks < kQThreads / 16 ? blocks : kQThreads / 16;
+  const dim3 threads(16 * across, kQThreads / (16 * across));
+  const dim3 grid((rows + threads.y - 1) / threads.y, (blocks + across - 1) / across);
+  if (grid.y > 65535) return cudaErrorInvalidValue;
+  MSCCL_BY_ELEM(elem, (quantize_rows_kernel<T><<<grid, threads, 0, stream>>>(static_cast<const T*>(x), ldx, static_cast<uint8_t*>(q), scales,
+                                                                          rows, k, s_row, s_block)));
   return cudaGetLastError();
 }
 
