@@ -7,9 +7,9 @@
 // the device only: every CTA derives the same list of tiles from the offsets, so nothing is copied to the host.
 //
 // The weights are the M operand and the rows of the group the N operand of the MMA: 256 features (of a CTA pair, cta_group::2)
-// by BN rows.  The last tile of a group is then padded to a multiple of BN = 64 .. 256 rows instead of 256, and a decode batch
-// streams the weights through tiles of 64 rows.  Rows of a tile that belong to the next group only reach columns of the accumulator
-// that are not stored, whatever they hold.  What is left of both operands behind the reduction dimension reads as zero.
+// by up to BN = 64 or 256 rows, and the last tile of a group is only as wide as its rows need, in steps of 32: N is a field of the
+// instruction.  (With tiles of 256 rows throughout, 8192 rows over 7 groups were padded by 11 %.)  Rows of a tile that belong to the
+// next group only reach columns of the accumulator that are not stored, whatever they hold.  What is left of both operands behind the reduction dimension reads as zero.
 //
 // The accumulator holds a feature per lane and a row per column; the epilogue transposes it (transpose_chunk).
 //
@@ -37,6 +37,7 @@ constexpr int kGABytes = BM * BK * 2;            // this CTA's 128 features: 16 
 constexpr int kGSmemLimit = 220 * 1024;
 
 template <int BN> struct Geometry {
+  static constexpr int kPiece = 32 * BK * 2;                 // rows of the last tile of a group come in pieces of 32 per CTA
   static constexpr int kBBytes = BN / 2 * BK * 2;
   static constexpr int kStageBytes = kGABytes + kBBytes;
   static constexpr int kFit = (kGSmemLimit - 2048) / kStageBytes;
@@ -56,7 +57,8 @@ struct GroupedArgs {
 
 template <int BN, bool MN_MAJOR, bool BF16>
 __global__ void __launch_bounds__(kGThreads, 1)
-grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const GroupedArgs g) {
+grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                    const __grid_constant__ CUtensorMap map_piece, const GroupedArgs g) {
   using Geo = Geometry<BN>;
   constexpr int S = Geo::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -90,6 +92,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     mbar_fence_init();
     prefetch_tensormap(&map_w);
     prefetch_tensormap(&map_x);
+    prefetch_tensormap(&map_piece);
   }
   if (warp == 1) tmem_alloc_pair(tmem_slot, Geo::kTmemCols);
   if (warp == 2) build_groups(table, g.offsets, g.groups, g.rows, [&](int rows) { return (rows + BN - 1) / BN * f_tiles; });
@@ -100,13 +103,14 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   const bool skip = ld_shared_cluster_u32(map_to_cta(smem_u32(&s_skip), 0)) != 0;
   const int num_tiles = table.tile_start[g.groups];
 
-  // tile -> group e, first row and first feature; e only moves forward
-  auto locate = [&](int tile, int& e, int& row, int& feature) {
+  // tile -> group e, first row, rows (a multiple of 32) and first feature; e only moves forward
+  auto locate = [&](int tile, int& e, int& row, int& width, int& feature) {
     while (tile >= table.tile_start[e + 1]) ++e;
     const int rows = table.row_start[e + 1] - table.row_start[e];
     int tm, tn;
     tile_coords(tile - table.tile_start[e], (rows + BN - 1) / BN, f_tiles, kGroupTileRows / BN, tm, tn);
     row = table.row_start[e] + tm * BN;
+    width = min(BN, (table.row_start[e + 1] - row + 31) / 32 * 32);
     feature = tn * 2 * BM;
   };
 
@@ -118,9 +122,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = first; tile < num_tiles && ok; tile += step) {
-        int row, feature;
-        locate(tile, e, row, feature);
-        row += static_cast<int>(rank) * (BN / 2);
+        int row, width, feature;
+        locate(tile, e, row, width, feature);
+        const int pieces = (width / 2 + 31) / 32;      // of this CTA's width / 2 rows
+        const uint32_t bytes = kGABytes + (width == BN ? Geo::kBBytes : pieces * Geo::kPiece);
+        row += static_cast<int>(rank) * (width / 2);
         feature += static_cast<int>(rank) * BM;
         for (int kb = 0; kb < k_blocks; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) {
@@ -129,7 +135,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             break;
           }
           uint8_t* a_dst = stage_base + static_cast<size_t>(stage) * Geo::kStageBytes;
-          if (leader) mbar_expect_tx(&full_bar[stage], 2 * Geo::kStageBytes);
+          if (leader) mbar_expect_tx(&full_bar[stage], 2 * bytes);
           const uint32_t bar = map_to_cta(smem_u32(&full_bar[stage]), 0);
           if (MN_MAJOR) {
             tma_pair_3d(a_dst, &map_w, bar, feature, kb * BK, e);
@@ -137,7 +143,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
           } else {
             tma_pair_3d(a_dst, &map_w, bar, kb * BK, feature, e);
           }
-          tma_pair_2d(a_dst + kGABytes, &map_x, bar, kb * BK, row);
+          if (width == BN) {
+            tma_pair_2d(a_dst + kGABytes, &map_x, bar, kb * BK, row);
+          } else {
+            for (int p = 0; p < pieces; ++p) tma_pair_2d(a_dst + kGABytes + p * Geo::kPiece, &map_piece, bar, kb * BK, row + 32 * p);
+          }
           if (++stage == S) { stage = 0; phase ^= 1; }
         }
       }
@@ -145,11 +155,14 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     }
   } else if (warp == 1) {
     if (leader && elect_one()) {
-      constexpr uint32_t idesc = idesc_16bit(BF16, 2 * BM, BN) | (MN_MAJOR ? kIdescTransA : 0u);
-      int stage = 0, acc = 0;
+      constexpr uint32_t idesc_rest = idesc_16bit(BF16, 2 * BM, 0) | (MN_MAJOR ? kIdescTransA : 0u);
+      int stage = 0, acc = 0, e = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       for (int tile = first; tile < num_tiles && ok; tile += step) {
+        int row, width, feature;
+        locate(tile, e, row, width, feature);
+        const uint32_t idesc = idesc_rest | static_cast<uint32_t>(width >> 3) << 17;
         if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1, abort_flag)) {
           gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 1, acc);
           break;
@@ -182,8 +195,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     int acc = 0, e = 0;
     uint32_t acc_phase = 0;
     for (int tile = first; tile < num_tiles; tile += step) {
-      int row, feature;
-      locate(tile, e, row, feature);
+      int row, width, feature;
+      locate(tile, e, row, width, feature);
       const int row_end = table.row_start[e + 1];
       bool ok = mbar_wait_warp(&acc_full[acc], acc_phase, abort_flag);
       if (!ok) {
@@ -231,7 +244,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 }
 
 template <int BN, bool MN_MAJOR, bool BF16>
-cudaError_t launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const GroupedArgs& g, int most_tiles, cudaStream_t stream) {
+cudaError_t launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const CUtensorMap& map_piece, const GroupedArgs& g, int most_tiles, cudaStream_t stream) {
   static int cached[64] = {};
   auto kernel = grouped_gemm_kernel<BN, MN_MAJOR, BF16>;
   int dev = 0;
@@ -245,20 +258,21 @@ cudaError_t launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const Gro
     if (clusters <= 0) return cudaErrorLaunchOutOfResources;
     cached[dev] = clusters;
   }
-  return launch_pairs_threads(kernel, Geometry<BN>::kSmem, most_tiles < cached[dev] ? most_tiles : cached[dev], kGThreads, stream, map_w, map_x, g);
+  return launch_pairs_threads(kernel, Geometry<BN>::kSmem, most_tiles < cached[dev] ? most_tiles : cached[dev], kGThreads, stream, map_w, map_x,
+                              map_piece, g);
 }
 
 template <int BN>
-cudaError_t launch_by_type(bool mn_major, bool bf16, const CUtensorMap& map_w, const CUtensorMap& map_x, const GroupedArgs& g, int most_tiles,
+cudaError_t launch_by_type(bool mn_major, bool bf16, const CUtensorMap& map_w, const CUtensorMap& map_x, const CUtensorMap& map_piece, const GroupedArgs& g, int most_tiles,
                            cudaStream_t stream) {
-  if (mn_major) return bf16 ? launch<BN, true, true>(map_w, map_x, g, most_tiles, stream) : launch<BN, true, false>(map_w, map_x, g, most_tiles, stream);
-  return bf16 ? launch<BN, false, true>(map_w, map_x, g, most_tiles, stream) : launch<BN, false, false>(map_w, map_x, g, most_tiles, stream);
+  if (mn_major) return bf16 ? launch<BN, true, true>(map_w, map_x, map_piece, g, most_tiles, stream) : launch<BN, true, false>(map_w, map_x, map_piece, g, most_tiles, stream);
+  return bf16 ? launch<BN, false, true>(map_w, map_x, map_piece, g, most_tiles, stream) : launch<BN, false, false>(map_w, map_x, map_piece, g, most_tiles, stream);
 }
 
 }  // namespace
 
 // w: [groups, n, k] (pitch ldw, matrix stride lde, elements); x: [rows, k] and out: [rows, n], or with `backward` x: [rows, n]
-// (dy) and out: [rows, k].  n % 8 == 0, k % 8 == 0, everything 16-byte aligned.  bn: 64, 128 or 256 rows per tile.
+// (dy) and out: [rows, k].  n % 8 == 0, k % 8 == 0, everything 16-byte aligned.  bn: 64 or 256 rows per tile.
 cudaError_t launch_grouped_gemm(const void* x, long long ldx, const void* w, long long ldw, long long lde, const int* offsets, void* out,
                                 long long ldo, int rows, int groups, int n, int k, bool backward, int elem, int bn, bool zero_rest,
                                 int* error_words, cudaStream_t stream) {
@@ -282,7 +296,9 @@ cudaError_t launch_grouped_gemm(const void* x, long long ldx, const void* w, lon
   const uint64_t x_dims[2] = {static_cast<uint64_t>(g.reduction), static_cast<uint64_t>(rows)};
   const uint64_t x_strides[1] = {static_cast<uint64_t>(ldx) * 2};
   const uint32_t x_box[2] = {64, static_cast<uint32_t>(bn / 2)};
+  const uint32_t piece_box[2] = {64, 32};
   const CUtensorMap map_x = make_swizzled_map(x, 2, 2, x_dims, x_strides, x_box);
+  const CUtensorMap map_piece = make_swizzled_map(x, 2, 2, x_dims, x_strides, piece_box);
   // as many tiles as there can be: every group may end inside one
   const long long f_tiles = (g.features + 2 * BM - 1) / (2 * BM), active = groups < rows ? groups : rows;
   const long long most = f_tiles * (rows / bn + active);
@@ -290,9 +306,8 @@ cudaError_t launch_grouped_gemm(const void* x, long long ldx, const void* w, lon
   const int most_tiles = most < 1 ? 1 : static_cast<int>(most);
   const bool bf16 = elem == kElemBF16;
   switch (bn) {
-    case 64: return launch_by_type<64>(backward, bf16, map_w, map_x, g, most_tiles, stream);
-    case 128: return launch_by_type<128>(backward, bf16, map_w, map_x, g, most_tiles, stream);
-    case 256: return launch_by_type<256>(backward, bf16, map_w, map_x, g, most_tiles, stream);
+    case 64: return launch_by_type<64>(backward, bf16, map_w, map_x, map_piece, g, most_tiles, stream);
+    case 256: return launch_by_type<256>(backward, bf16, map_w, map_x, map_piece, g, most_tiles, stream);
     default: return cudaErrorInvalidValue;
   }
 }

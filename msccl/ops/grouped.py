@@ -17,11 +17,10 @@ _TYPES = (torch.bfloat16, torch.float16)
 
 
 def _tile_rows(rows, experts):
-    """Rows per tile from the mean size of a group (the sizes themselves are on the device).  Microseconds with 64 / 128 / 256 rows,
-    forward: 32 rows x 8 experts of 14336 x 4096 165 / 166 / 186; 4096 x 64 of 1024 x 2048 69 / 69 / 74; 1024 x 8 of 4096 x 4096 76 / 68 /
-    70; 8192 x 8 of 14336 x 4096 1014 / 734 / 693."""
-    mean = rows / max(1, min(rows, experts))
-    return 64 if mean <= 48 else 128 if mean <= 256 else 256
+    """The most rows of a tile, from the mean size of a group (the sizes themselves are on the device): tiles of 64 leave room for more
+    of the weights on their way, tiles of 256 read them less often.  Microseconds with 64 / 256 rows, forward: 32 rows x 8 experts of
+    14336 x 4096 164 / 178; 4096 x 64 of 1024 x 2048 72 / 72; 1024 x 8 of 4096 x 4096 80 / 72; 8192 x 8 of 14336 x 4096 1115 / 696."""
+    return 64 if rows <= 48 * min(rows, experts) else 256
 
 
 def _check_experts(experts):
