@@ -7,6 +7,8 @@ large ones): no copy into a communication buffer and none back.
 """
 import torch
 
+from msccl.ops.grad_norm import clip_grad_norm
+
 
 class FlatGradients:
     def __init__(self, parameters, allocate, dtype=None, bucket_bytes=1 << 30):
@@ -51,3 +53,9 @@ class FlatGradients:
             all_reduce(flat)
             if average:
                 flat.div_(world)
+
+    def clip_grad_norm(self, max_norm, reduce=None):
+        """Scale all gradients by ``min(1, max_norm / (norm + 1e-6))`` in place, ``norm`` their global 2-norm, and return it
+        (``msccl.ops.grad_norm.clip_grad_norm`` on the buckets; the slots' padding is zero).  After ``all_reduce_gradients`` every rank
+        has the same gradients and needs no ``reduce``."""
+        return clip_grad_norm([flat for flat, _ in self.buckets], max_norm, reduce=reduce)

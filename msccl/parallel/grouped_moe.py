@@ -1,0 +1,62 @@
+"""Mixture-of-experts layer on one GPU without a capacity, trained or served: every token copy reaches its expert, whatever the
+router does.  ``ExpertParallelMoE`` shards experts over GPUs and is forward only; this layer holds all of its experts and is the one
+to train data-parallel (``FlatGradients`` takes its parameters, sums and clips their gradients).
+"""
+import torch
+
+from msccl.ops.fp8_block import grouped_gemm_fp8_block, quantize_fp8_block, quantize_fp8_block_weight
+from msccl.ops.grouped import grouped_gemm
+from msccl.ops.moe import route_top_k
+from msccl.ops.moe_rows import combine_rows, gather_rows, sort_copies
+
+
+class GroupedMoE(torch.nn.Module):
+    """``y[t] = sum_j p[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t]))`` over the ``topk`` experts ``e`` of token ``t``, ``p`` the softmax
+    over their router logits.
+
+    ``forward`` takes any number of tokens (one at least), [tokens, hidden] in the layer's dtype, and is differentiable in ``x``, the
+    router and the experts.  ``quantize()`` makes the fp8 form of the experts; ``forward(x, precision='fp8')`` then runs on it, without
+    gradients.  hidden and ffn: multiples of 8 (16 for fp8)."""
+
+    def __init__(self, hidden, ffn, num_experts, topk=2, device='cuda', dtype=torch.bfloat16, std=0.02, seed=0):
+        super().__init__()
+        self.hidden, self.ffn, self.num_experts, self.topk = hidden, ffn, num_experts, topk
+        gen = torch.Generator(device=device).manual_seed(seed)
+
+        def mk(*shape):
+            return torch.nn.Parameter((torch.randn(*shape, device=device, generator=gen) * std).to(dtype))
+        self.w_router = mk(num_experts, hidden)
+        self.w_gate_up = mk(num_experts, 2 * ffn, hidden)        # the gate's rows, then the up projection's
+        self.w_down = mk(num_experts, hidden, ffn)
+        self._fp8 = None
+
+    def quantize(self):
+        """Quantise the experts as they are now (blocks of 128 x 128, ``msccl.ops.fp8_block``)."""
+        self._fp8 = quantize_fp8_block_weight(self.w_gate_up.detach()) + quantize_fp8_block_weight(self.w_down.detach())
+        return self
+
+    def _experts(self, xs, offsets):
+        gate, up = grouped_gemm(xs, self.w_gate_up, offsets).split(self.ffn, 1)
+        return grouped_gemm(torch.nn.functional.silu(gate) * up, self.w_down, offsets)
+
+    def _experts_fp8(self, xs, offsets):
+        w_gate_up, s_gate_up, w_down, s_down = self._fp8
+        gate, up = grouped_gemm_fp8_block(*quantize_fp8_block(xs), w_gate_up, s_gate_up, offsets).split(self.ffn, 1)
+        return grouped_gemm_fp8_block(*quantize_fp8_block(torch.nn.functional.silu(gate) * up), w_down, s_down, offsets)
+
+    def forward(self, x, gate_logits=None, precision='bf16'):
+        if precision not in ('bf16', 'fp8'):
+            raise ValueError(f"precision is 'bf16' or 'fp8' (got {precision!r})")
+        if precision == 'fp8':
+            if self._fp8 is None:
+                raise RuntimeError('call quantize() before a forward pass in fp8')
+            with torch.no_grad():
+                return self._forward(x, gate_logits, self._experts_fp8)
+        return self._forward(x, gate_logits, self._experts)
+
+    def _forward(self, x, gate_logits, run_experts):
+        if gate_logits is None:
+            gate_logits = x @ self.w_router.t()
+        experts, weights = route_top_k(gate_logits, self.topk)
+        order = sort_copies(experts, self.num_experts)
+        return combine_rows(run_experts(gather_rows(x, order), order.offsets), weights, order)
