@@ -140,15 +140,38 @@ __device__ __forceinline__ void zero_rest_rows(const GroupTable& table, const FA
   }
 }
 
-// One row's columns [column, column + 2 * PAIRS) as bf16, as far as the result has them (multiples of 8).
+// The columns [column, column + 2 * PAIRS) of 32 rows, one per lane, as bf16, as far as the result has them (multiples of 8 columns).
+// PAIRS / 4 lanes exchange their 16-byte pieces first, so that they store one stretch of a row instead of a piece of one row each.
 template <int PAIRS>
-__device__ __forceinline__ void store_row(const FArgs& g, long long row, int column, const float2 (&sum)[PAIRS]) {
-  __nv_bfloat16* out = g.out + row * g.ldo + column;
+__device__ __forceinline__ void store_rows(const FArgs& g, long long row0, int rows, int column, const float2 (&sum)[PAIRS]) {
+  constexpr int P = PAIRS / 4;                   // pieces of a row: 2, 4 or 8
+  const int lane = threadIdx.x % 32;
+  uint4 v[P];
 #pragma unroll
-  for (int c = 0; c < PAIRS; c += 4)
-    if (column + 2 * c < g.n)
-      *reinterpret_cast<uint4*>(out + 2 * c) = make_uint4(pack_bf16(sum[c].x, sum[c].y), pack_bf16(sum[c + 1].x, sum[c + 1].y),
-                                                          pack_bf16(sum[c + 2].x, sum[c + 2].y), pack_bf16(sum[c + 3].x, sum[c + 3].y));
+  for (int i = 0; i < P; ++i)
+    v[i] = make_uint4(pack_bf16(sum[4 * i].x, sum[4 * i].y), pack_bf16(sum[4 * i + 1].x, sum[4 * i + 1].y),
+                      pack_bf16(sum[4 * i + 2].x, sum[4 * i + 2].y), pack_bf16(sum[4 * i + 3].x, sum[4 * i + 3].y));
+  // transpose P x P pieces among P lanes: afterwards v[i] is piece lane % P of row (lane / P) * P + i
+#pragma unroll
+  for (int bit = 1; bit < P; bit <<= 1) {
+    const bool up = (lane & bit) != 0;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      if (i & bit) continue;
+      const uint4 give = up ? v[i] : v[i | bit];
+      const uint4 got = make_uint4(__shfl_xor_sync(kFullMask, give.x, bit), __shfl_xor_sync(kFullMask, give.y, bit),
+                                   __shfl_xor_sync(kFullMask, give.z, bit), __shfl_xor_sync(kFullMask, give.w, bit));
+      if (up) v[i] = got; else v[i | bit] = got;
+    }
+  }
+  const int c = column + lane % P * 8, first = lane / P * P;
+  if (c >= g.n) return;
+  __nv_bfloat16* out = g.out + (row0 + first) * g.ldo + c;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    if (first + i < rows) *reinterpret_cast<uint4*>(out) = v[i];
+    out += g.ldo;
+  }
 }
 
 constexpr int kFThreads = 320;                   // 0 producer, 1 MMA, 2..9 scaling and epilogue
@@ -356,7 +379,7 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         if (++acc == ACCS) { acc = 0; acc_phase ^= 1; }
         }
       }
-      if (ok && lane < left) store_row(g, row, column, sum);
+      if (ok && left > 0) store_rows(g, row - lane, left, column, sum);
     }
     if (g.zero_rest && !skip) zero_rest_rows(table, g, blockIdx.x * kFEpilogueWarps + warp - 2, gridDim.x * kFEpilogueWarps);
   }
