@@ -575,11 +575,13 @@ PYBIND11_MODULE(_msccl_native, m) {
   });
   // Rows around the experts: elem 0 = fp32, 1 = bf16, 2 = fp16; pointers that may be 0 are said to be in moe_rows.cu.
   m.def("sort_copies", [](uintptr_t expert_of, bool wide_ids, long long n, int experts, uintptr_t sorted_copy, uintptr_t expert_start,
-                          uintptr_t position, uintptr_t stream) {
+                          uintptr_t position, uintptr_t workspace, uintptr_t stream) {
     check_rt(msccl::sm100::launch_sort_copies(reinterpret_cast<const void*>(expert_of), wide_ids, n, experts, reinterpret_cast<int*>(sorted_copy),
-                                              reinterpret_cast<int*>(expert_start), reinterpret_cast<int*>(position), as_stream(stream)),
+                                              reinterpret_cast<int*>(expert_start), reinterpret_cast<int*>(position), reinterpret_cast<int*>(workspace),
+                                              as_stream(stream)),
              "launch of the copy sort kernel");
   });
+  m.def("sort_copies_workspace", &msccl::sm100::sort_copies_workspace);
   m.def("scatter_rows", [](uintptr_t x, long long ldx, uintptr_t out, uintptr_t position, uintptr_t rows_kept, int tokens, int topk, int hidden,
                            int elem, uintptr_t stream) {
     check_rt(msccl::sm100::launch_scatter_rows(reinterpret_cast<const void*>(x), ldx, reinterpret_cast<void*>(out),

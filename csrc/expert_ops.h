@@ -14,7 +14,8 @@ enum ElemType : int { kElemF32 = 0, kElemBF16 = 1, kElemF16 = 2 };
 
 // ---- rows around the experts
 cudaError_t launch_sort_copies(const void* expert_of, bool wide_ids, long long n, int experts, int* sorted_copy, int* expert_start,
-                               int* position, cudaStream_t stream);
+                               int* position, int* workspace, cudaStream_t stream);
+long long sort_copies_workspace(long long n, int experts);
 cudaError_t launch_scatter_rows(const void* x, long long ldx, void* out, const int* position, const int* rows_kept, int tokens, int topk,
                                 int hidden, int elem, cudaStream_t stream);
 cudaError_t launch_combine_rows(const void* ys, long long ldy, const float* weights, void* out, const int* position, const int* rows_kept,

@@ -14,6 +14,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "expert_ops.h"
 
@@ -28,13 +29,36 @@ constexpr int kSortMaxExperts = 512;
 constexpr int kRowsMaxTopk = 8;
 constexpr int kRowThreads = 256;
 
-// Every CTA orders its own 1024 copies.  It needs the expert counts of all copies and of the copies before its own: it counts
-// them itself (n ids from L2, 131072 at most 0.5 MB) instead of waiting for other CTAs, so that one launch does and nothing has
-// to be cleared.  Counts are integers: the order of the shared-memory additions does not show.
+// Every CTA orders its own 1024 copies.  It needs the expert counts of all copies and of the copies before its own.  Up to 32 CTAs
+// count them themselves (n ids from L2) instead of waiting for other CTAs, so that one launch does and nothing has to be cleared; with
+// more a launch before this one has written the counts of each CTA's copies to `counts` (131072 copies, 256 experts: 144 us
+// without, under 17 with it).  Counts are integers: the order of the shared-memory additions does not show.
+constexpr int kSortAlone = 32;
+
+template <typename Id>
+__device__ __forceinline__ int bucket_of(const Id* __restrict__ expert_of, int i, int n, int experts) {
+  if (i >= n) return -1;
+  const Id id = expert_of[i];
+  return id >= 0 && id < static_cast<Id>(experts) ? static_cast<int>(id) : experts;
+}
+
 template <typename Id>
 __global__ void __launch_bounds__(kSortThreads, 1)
-sort_copies_kernel(const Id* __restrict__ expert_of, int n, int experts, int* __restrict__ sorted_copy, int* __restrict__ expert_start,
-                   int* __restrict__ position) {
+count_copies_kernel(const Id* __restrict__ expert_of, int n, int experts, int* __restrict__ counts) {
+  __shared__ int here[kSortMaxExperts + 1];
+  for (int i = threadIdx.x; i <= experts; i += kSortThreads) here[i] = 0;
+  __syncthreads();
+  const int e = bucket_of(expert_of, blockIdx.x * kSortThreads + threadIdx.x, n, experts);
+  const unsigned int same = __match_any_sync(0xffffffffu, e);
+  if (e >= 0 && (same & ((1u << (threadIdx.x % 32)) - 1u)) == 0) atomicAdd(&here[e], __popc(same));
+  __syncthreads();
+  for (int i = threadIdx.x; i <= experts; i += kSortThreads) counts[static_cast<long long>(blockIdx.x) * (experts + 1) + i] = here[i];
+}
+
+template <typename Id>
+__global__ void __launch_bounds__(kSortThreads, 1)
+sort_copies_kernel(const Id* __restrict__ expert_of, int n, int experts, const int* __restrict__ counts, int* __restrict__ sorted_copy,
+                   int* __restrict__ expert_start, int* __restrict__ position) {
   __shared__ int total[kSortMaxExperts + 1], before[kSortMaxExperts + 1], start[kSortMaxExperts + 2];
   __shared__ unsigned short in_warp[kSortWarps][kSortMaxExperts + 1];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -45,21 +69,32 @@ sort_copies_kernel(const Id* __restrict__ expert_of, int n, int experts, int* __
   const int own = blockIdx.x * kSortThreads;
   int my_bucket = -1;
   unsigned int my_rank = 0;
-  for (int base = 0; base < n; base += kSortThreads) {
-    const int i = base + threadIdx.x;
-    int e = -1;
-    if (i < n) {
-      const Id id = expert_of[i];
-      e = id >= 0 && id < static_cast<Id>(experts) ? static_cast<int>(id) : experts;
+  if (counts != nullptr) {
+    my_bucket = bucket_of(expert_of, own + static_cast<int>(threadIdx.x), n, experts);
+    const unsigned int same = __match_any_sync(0xffffffffu, my_bucket);
+    my_rank = __popc(same & ((1u << lane) - 1u));
+    if (my_bucket >= 0 && my_rank == 0) in_warp[warp][my_bucket] = static_cast<unsigned short>(__popc(same));
+    // two threads for each bucket: CTAs before this one, and the others
+    for (int i = threadIdx.x; i < 2 * buckets; i += kSortThreads) {
+      const int e = i % buckets, lo = i < buckets ? 0 : blockIdx.x, hi = i < buckets ? blockIdx.x : gridDim.x;
+      int sum = 0;
+#pragma unroll 8
+      for (int c = lo; c < hi; ++c) sum += counts[static_cast<long long>(c) * buckets + e];
+      if (i < buckets) before[e] = sum;
+      atomicAdd(&total[e], sum);
     }
-    const unsigned int same = __match_any_sync(0xffffffffu, e);
-    const unsigned int rank = __popc(same & ((1u << lane) - 1u));
-    if (e >= 0 && rank == 0) {
-      atomicAdd(&total[e], __popc(same));
-      if (base < own) atomicAdd(&before[e], __popc(same));
-      if (base == own) in_warp[warp][e] = static_cast<unsigned short>(__popc(same));
+  } else {
+    for (int base = 0; base < n; base += kSortThreads) {
+      const int e = bucket_of(expert_of, base + static_cast<int>(threadIdx.x), n, experts);
+      const unsigned int same = __match_any_sync(0xffffffffu, e);
+      const unsigned int rank = __popc(same & ((1u << lane) - 1u));
+      if (e >= 0 && rank == 0) {
+        atomicAdd(&total[e], __popc(same));
+        if (base < own) atomicAdd(&before[e], __popc(same));
+        if (base == own) in_warp[warp][e] = static_cast<unsigned short>(__popc(same));
+      }
+      if (base == own) { my_bucket = e; my_rank = rank; }
     }
-    if (base == own) { my_bucket = e; my_rank = rank; }
   }
   __syncthreads();
   if (warp == 0) {                             // exclusive prefix of the totals
@@ -168,88 +203,108 @@ scatter_rows_kernel(const T* __restrict__ x, long long ldx, T* __restrict__ out,
   }
 }
 
-template <typename T, bool WEIGHTED>
+// K >= topk copies and V vectors of a row per thread and step, K * V loads in flight (one vector of a token with two copies kept HBM at
+// 4.0 TB/s).
+template <typename T, int K, bool WEIGHTED>
 __global__ void __launch_bounds__(kRowThreads)
 combine_rows_kernel(const T* __restrict__ ys, long long ldy, const float* __restrict__ weights, T* __restrict__ out,
                     const int* __restrict__ position, const int* __restrict__ rows_kept, int topk, int hidden) {
-  constexpr int N = Pack<T>::kN;
+  constexpr int N = Pack<T>::kN, V = K <= 2 ? 4 / K : 1;
   const long long t = blockIdx.x;
   const int kept = *rows_kept, vecs = hidden / N;
-  int rows[kRowsMaxTopk];
-  float w[kRowsMaxTopk];
+  int rows[K];
+  float w[K];
 #pragma unroll
-  for (int j = 0; j < kRowsMaxTopk; ++j) {
+  for (int j = 0; j < K; ++j) {
     rows[j] = j < topk ? position[t * topk + j] : kept;
     w[j] = WEIGHTED && j < topk ? weights[t * topk + j] : 1.0f;
   }
-  for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
-    uint4 val[kRowsMaxTopk];
+  for (int v0 = threadIdx.x; v0 < vecs; v0 += V * blockDim.x) {
+    uint4 val[V][K];
 #pragma unroll
-    for (int j = 0; j < kRowsMaxTopk; ++j)
-      if (rows[j] < kept) val[j] = reinterpret_cast<const uint4*>(ys + static_cast<long long>(rows[j]) * ldy)[v];
-    float sum[N];
+    for (int i = 0; i < V; ++i)
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum[i] = 0.0f;
+      for (int j = 0; j < K; ++j)
+        if (rows[j] < kept && v0 + i * blockDim.x < vecs)
+          val[i][j] = reinterpret_cast<const uint4*>(ys + static_cast<long long>(rows[j]) * ldy)[v0 + i * blockDim.x];
 #pragma unroll
-    for (int j = 0; j < kRowsMaxTopk; ++j)
-      if (rows[j] < kept) {
-        float f[N];
-        Pack<T>::load(val[j], f);
+    for (int i = 0; i < V; ++i) {
+      if (v0 + i * blockDim.x >= vecs) break;
+      float sum[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum[i] = WEIGHTED ? fmaf(w[j], f[i], sum[i]) : sum[i] + f[i];
-      }
-    reinterpret_cast<uint4*>(out + t * hidden)[v] = Pack<T>::store(sum);
+      for (int c = 0; c < N; ++c) sum[c] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < K; ++j)
+        if (rows[j] < kept) {
+          float f[N];
+          Pack<T>::load(val[i][j], f);
+#pragma unroll
+          for (int c = 0; c < N; ++c) sum[c] = WEIGHTED ? fmaf(w[j], f[c], sum[c]) : sum[c] + f[c];
+        }
+      reinterpret_cast<uint4*>(out + t * hidden)[v0 + i * blockDim.x] = Pack<T>::store(sum);
+    }
   }
 }
 
-template <typename T>
+template <typename T, int K>
 __global__ void __launch_bounds__(kRowThreads)
 combine_backward_kernel(const T* __restrict__ dy, long long lddy, const T* __restrict__ ys, long long ldy, const float* __restrict__ weights,
                         T* __restrict__ dys, float* __restrict__ dweights, const int* __restrict__ position,
                         const int* __restrict__ rows_kept, int topk, int hidden) {
-  constexpr int N = Pack<T>::kN;
-  __shared__ float partial[kRowThreads / 32][kRowsMaxTopk];
+  constexpr int N = Pack<T>::kN, V = K <= 2 ? 2 : 1;
+  __shared__ float partial[kRowThreads / 32][K];
   const long long t = blockIdx.x;
   const int kept = *rows_kept, vecs = hidden / N;
-  int rows[kRowsMaxTopk];
-  float w[kRowsMaxTopk], dot[kRowsMaxTopk];
+  int rows[K];
+  float w[K], dot[K];
 #pragma unroll
-  for (int j = 0; j < kRowsMaxTopk; ++j) {
+  for (int j = 0; j < K; ++j) {
     rows[j] = j < topk ? position[t * topk + j] : kept;
     w[j] = j < topk ? weights[t * topk + j] : 0.0f;
     dot[j] = 0.0f;
   }
   const uint4* src = reinterpret_cast<const uint4*>(dy + t * lddy);
-  for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
-    float g[N];
-    Pack<T>::load(src[v], g);
-    uint4 val[kRowsMaxTopk];
+  for (int v0 = threadIdx.x; v0 < vecs; v0 += V * blockDim.x) {
+    uint4 gv[V], val[V][K];
 #pragma unroll
-    for (int j = 0; j < kRowsMaxTopk; ++j)
-      if (rows[j] < kept && dweights != nullptr) val[j] = reinterpret_cast<const uint4*>(ys + static_cast<long long>(rows[j]) * ldy)[v];
+    for (int i = 0; i < V; ++i) {
+      const int v = v0 + i * blockDim.x;
+      if (v >= vecs) break;
+      gv[i] = src[v];
 #pragma unroll
-    for (int j = 0; j < kRowsMaxTopk; ++j) {
-      if (j >= topk) continue;
-      float f[N];
-      if (rows[j] < kept) {
-        if (dweights != nullptr) {
-          Pack<T>::load(val[j], f);
+      for (int j = 0; j < K; ++j)
+        if (rows[j] < kept && dweights != nullptr) val[i][j] = reinterpret_cast<const uint4*>(ys + static_cast<long long>(rows[j]) * ldy)[v];
+    }
 #pragma unroll
-          for (int i = 0; i < N; ++i) dot[j] = fmaf(f[i], g[i], dot[j]);
+    for (int i = 0; i < V; ++i) {
+      const int v = v0 + i * blockDim.x;
+      if (v >= vecs) break;
+      float g[N];
+      Pack<T>::load(gv[i], g);
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        if (j >= topk) continue;
+        float f[N];
+        if (rows[j] < kept) {
+          if (dweights != nullptr) {
+            Pack<T>::load(val[i][j], f);
+#pragma unroll
+            for (int c = 0; c < N; ++c) dot[j] = fmaf(f[c], g[c], dot[j]);
+          }
+#pragma unroll
+          for (int c = 0; c < N; ++c) f[c] = w[j] * g[c];
+        } else {
+#pragma unroll
+          for (int c = 0; c < N; ++c) f[c] = 0.0f;
         }
-#pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = w[j] * g[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = 0.0f;
+        if (dys != nullptr) reinterpret_cast<uint4*>(dys + static_cast<long long>(rows[j]) * hidden)[v] = Pack<T>::store(f);
       }
-      if (dys != nullptr) reinterpret_cast<uint4*>(dys + static_cast<long long>(rows[j]) * hidden)[v] = Pack<T>::store(f);
     }
   }
   if (dweights == nullptr) return;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 #pragma unroll
-  for (int j = 0; j < kRowsMaxTopk; ++j) {
+  for (int j = 0; j < K; ++j) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], off);
     if (lane == 0) partial[warp][j] = dot[j];
@@ -276,17 +331,25 @@ int row_threads(int hidden, int elem) {
 
 }  // namespace
 
+// Integers of workspace that launch_sort_copies needs.
+long long sort_copies_workspace(long long n, int experts) {
+  const long long ctas = (n + kSortThreads - 1) / kSortThreads;
+  return ctas > kSortAlone ? ctas * (experts + 1) : 0;
+}
+
 // expert_of: n ids (int32, or int64 with wide_ids).
 cudaError_t launch_sort_copies(const void* expert_of, bool wide_ids, long long n, int experts, int* sorted_copy, int* expert_start,
-                               int* position, cudaStream_t stream) {
+                               int* position, int* workspace, cudaStream_t stream) {
   if (n < 1 || n > (1 << 22) || experts < 1 || experts > kSortMaxExperts) return cudaErrorInvalidValue;
-  const int grid = static_cast<int>((n + kSortThreads - 1) / kSortThreads);
-  if (wide_ids)
-    sort_copies_kernel<long long><<<grid, kSortThreads, 0, stream>>>(static_cast<const long long*>(expert_of), static_cast<int>(n), experts,
-                                                                   sorted_copy, expert_start, position);
-  else
-    sort_copies_kernel<int><<<grid, kSortThreads, 0, stream>>>(static_cast<const int*>(expert_of), static_cast<int>(n), experts, sorted_copy,
-                                                             expert_start, position);
+  const int grid = static_cast<int>((n + kSortThreads - 1) / kSortThreads), count = static_cast<int>(n);
+  int* counts = sort_copies_workspace(n, experts) > 0 ? workspace : nullptr;
+  auto run = [&](auto* ids) {
+    using Id = std::remove_const_t<std::remove_pointer_t<decltype(ids)>>;
+    if (counts != nullptr) count_copies_kernel<Id><<<grid, kSortThreads, 0, stream>>>(ids, count, experts, counts);
+    sort_copies_kernel<Id><<<grid, kSortThreads, 0, stream>>>(ids, count, experts, counts, sorted_copy, expert_start, position);
+  };
+  if (wide_ids) run(static_cast<const long long*>(expert_of));
+  else run(static_cast<const int*>(expert_of));
   return cudaGetLastError();
 }
 
@@ -297,6 +360,12 @@ cudaError_t launch_sort_copies(const void* expert_of, bool wide_ids, long long n
     case kElemF16: { using T = __half; __VA_ARGS__; break; }            \
     default: return cudaErrorInvalidValue;                              \
   }
+
+#define MSCCL_BY_COPIES(topk, ...)                                      \
+  if (topk == 1) { constexpr int K = 1; __VA_ARGS__; }                  \
+  else if (topk == 2) { constexpr int K = 2; __VA_ARGS__; }             \
+  else if (topk <= 4) { constexpr int K = 4; __VA_ARGS__; }             \
+  else { constexpr int K = 8; __VA_ARGS__; }
 
 cudaError_t launch_scatter_rows(const void* x, long long ldx, void* out, const int* position, const int* rows_kept, int tokens, int topk,
                                 int hidden, int elem, cudaStream_t stream) {
@@ -311,13 +380,10 @@ cudaError_t launch_combine_rows(const void* ys, long long ldy, const float* weig
                                 int tokens, int topk, int hidden, int elem, cudaStream_t stream) {
   if (!rows_ok(tokens, topk, hidden, elem)) return cudaErrorInvalidValue;
   const int threads = row_threads(hidden, elem);
-  if (weights != nullptr) {
-    MSCCL_BY_ELEM(elem, (combine_rows_kernel<T, true><<<tokens, threads, 0, stream>>>(static_cast<const T*>(ys), ldy, weights, static_cast<T*>(out),
-                                                                                      position, rows_kept, topk, hidden)));
-  } else {
-    MSCCL_BY_ELEM(elem, (combine_rows_kernel<T, false><<<tokens, threads, 0, stream>>>(static_cast<const T*>(ys), ldy, weights, static_cast<T*>(out),
-                                                                                       position, rows_kept, topk, hidden)));
-  }
+  MSCCL_BY_ELEM(elem, MSCCL_BY_COPIES(topk, {
+    auto kernel = weights != nullptr ? combine_rows_kernel<T, K, true> : combine_rows_kernel<T, K, false>;
+    kernel<<<tokens, threads, 0, stream>>>(static_cast<const T*>(ys), ldy, weights, static_cast<T*>(out), position, rows_kept, topk, hidden);
+  }));
   return cudaGetLastError();
 }
 
@@ -326,9 +392,9 @@ cudaError_t launch_combine_backward(const void* dy, long long lddy, const void* 
                                     float* dweights, const int* position, const int* rows_kept, int tokens, int topk, int hidden,
                                     int elem, cudaStream_t stream) {
   if (!rows_ok(tokens, topk, hidden, elem)) return cudaErrorInvalidValue;
-  MSCCL_BY_ELEM(elem, (combine_backward_kernel<T><<<tokens, row_threads(hidden, elem), 0, stream>>>(
-                          static_cast<const T*>(dy), lddy, static_cast<const T*>(ys), ldy, weights, static_cast<T*>(dys), dweights, position,
-                          rows_kept, topk, hidden)));
+  MSCCL_BY_ELEM(elem, MSCCL_BY_COPIES(topk, (combine_backward_kernel<T, K><<<tokens, row_threads(hidden, elem), 0, stream>>>(
+                                               static_cast<const T*>(dy), lddy, static_cast<const T*>(ys), ldy, weights, static_cast<T*>(dys),
+                                               dweights, position, rows_kept, topk, hidden))));
   return cudaGetLastError();
 }
 

@@ -28,7 +28,7 @@ class CopyOrder(NamedTuple):
 
 
 def sort_copies(experts, num_experts, stream=None):
-    """Stable order of the copies ``experts`` [tokens, k] (int32 or int64) by expert, in one launch.  A copy whose id is outside
+    """Stable order of the copies ``experts`` [tokens, k] (int32 or int64) by expert, in one launch (two from 32768 copies on).  A copy whose id is outside
     ``[0, num_experts)`` is dropped: the gather gives it a row of zeros behind the last expert's, the combination ignores it."""
     if experts.dim() != 2 or experts.dtype not in (torch.int32, torch.int64):
         raise ValueError('experts must be a [tokens, k] int32 or int64 tensor')
@@ -41,10 +41,13 @@ def sort_copies(experts, num_experts, stream=None):
     index = check_devices(experts=experts)
     with on_stream(index, stream, (experts,)):
         experts = experts.contiguous()
+        native = load()
+        workspace = native.sort_copies_workspace(copies, num_experts)
         table = torch.empty(2 * copies + num_experts + 1, dtype=torch.int32, device=experts.device)
         sorted_copy, position, offsets = table.split((copies, copies, num_experts + 1))
-        load().sort_copies(experts.data_ptr(), experts.dtype == torch.int64, copies, num_experts, sorted_copy.data_ptr(),
-                           offsets.data_ptr(), position.data_ptr(), stream_handle(index))
+        counts = torch.empty(workspace, dtype=torch.int32, device=experts.device).data_ptr() if workspace else 0
+        native.sort_copies(experts.data_ptr(), experts.dtype == torch.int64, copies, num_experts, sorted_copy.data_ptr(),
+                           offsets.data_ptr(), position.data_ptr(), counts, stream_handle(index))
     return CopyOrder(sorted_copy, offsets, position.view(tokens, topk))
 
 
