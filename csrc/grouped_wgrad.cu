@@ -2,8 +2,8 @@
 //
 // Both operands are read as they lie in memory: the reduction runs over rows, so both are MN-major (64 features x 64 rows slabs of
 // 8 KB).  CTA pairs (cta_group::2) compute 256 x 256 tiles; a group without rows writes zeros.  x is the M operand, so that
-// the lanes of an accumulator run along k, the contiguous dimension of the result (dy as the M operand gave every lane a row of
-// its own to store to, 16 bytes at a time: 8 groups of 1024 rows, n = k = 4096, 432 us).
+// the lanes of an accumulator run along k, the contiguous dimension of the result.  8 groups of 1024 rows, n = k = 4096: 162 us, 1.70
+// PFLOP/s; of a few rows each the result's 2.5 TB/s of writes are the bound (3.7 us per tile).
 //
 // The reduction is ragged: the last 64-row block of a group also covers rows of the next group (or memory behind the last one, which
 // may hold anything).  Those rows have to be zero in both operands, since 0 times infinity is not 0.  So that block goes a way of

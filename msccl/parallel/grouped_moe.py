@@ -15,8 +15,8 @@ class GroupedMoE(torch.nn.Module):
     over their router logits.
 
     ``forward`` takes any number of tokens (one at least), [tokens, hidden] in the layer's dtype, and is differentiable in ``x``, the
-    router and the experts.  ``quantize()`` makes the fp8 form of the experts; ``forward(x, precision='fp8')`` then runs on it, without
-    gradients.  hidden and ffn: multiples of 8 (16 for fp8)."""
+    router and the experts.  ``quantize()`` makes the fp8 form of the experts (of a bf16 layer); ``forward(x, precision='fp8')`` then runs
+    on it, without gradients; the default runs in the layer's own type.  hidden and ffn: multiples of 8 (16 for fp8)."""
 
     def __init__(self, hidden, ffn, num_experts, topk=2, device='cuda', dtype=torch.bfloat16, std=0.02, seed=0):
         super().__init__()
@@ -31,7 +31,9 @@ class GroupedMoE(torch.nn.Module):
         self._fp8 = None
 
     def quantize(self):
-        """Quantise the experts as they are now (blocks of 128 x 128, ``msccl.ops.fp8_block``)."""
+        """Quantise the experts as they are now (blocks of 128 x 128, ``msccl.ops.fp8_block``).  Training goes on with the others."""
+        if self.w_down.dtype != torch.bfloat16:
+            raise ValueError(f'the fp8 products give bf16, the layer is {self.w_down.dtype}')
         self._fp8 = quantize_fp8_block_weight(self.w_gate_up.detach()) + quantize_fp8_block_weight(self.w_down.detach())
         return self
 
@@ -44,9 +46,9 @@ class GroupedMoE(torch.nn.Module):
         gate, up = grouped_gemm_fp8_block(*quantize_fp8_block(xs), w_gate_up, s_gate_up, offsets).split(self.ffn, 1)
         return grouped_gemm_fp8_block(*quantize_fp8_block(torch.nn.functional.silu(gate) * up), w_down, s_down, offsets)
 
-    def forward(self, x, gate_logits=None, precision='bf16'):
-        if precision not in ('bf16', 'fp8'):
-            raise ValueError(f"precision is 'bf16' or 'fp8' (got {precision!r})")
+    def forward(self, x, gate_logits=None, precision=None):
+        if precision not in (None, 'fp8'):
+            raise ValueError(f"precision is None (the layer's own) or 'fp8' (got {precision!r})")
         if precision == 'fp8':
             if self._fp8 is None:
                 raise RuntimeError('call quantize() before a forward pass in fp8')

@@ -23,7 +23,7 @@ def _reference(layer, x, experts, weights):
 
 
 def _rel(a, b):
-    return float((a.double() - b).norm() / b.norm())
+    return float((a.detach().double() - b.detach()).norm() / b.detach().norm())
 
 
 @pytest.mark.parametrize('tokens,hidden,ffn,experts,topk,dtype', [(1, 64, 128, 4, 2, torch.bfloat16), (100, 136, 72, 8, 3, torch.bfloat16),
@@ -92,6 +92,8 @@ def test_fp8_forward():
         layer(x, precision='fp8')
     with pytest.raises(ValueError):
         layer(x, precision='fp4')
+    with pytest.raises(ValueError):
+        GroupedMoE(64, 64, 2, dtype=torch.float16).quantize()
     layer.quantize()
     y8, y = layer(x, precision='fp8'), layer(x)
     check_gemm_errors()
@@ -108,13 +110,51 @@ def test_captured_forward_with_other_routing():
     gen = torch.Generator(device='cuda').manual_seed(2)
     x = torch.randn(40, 128, device='cuda', generator=gen).bfloat16()
     with torch.no_grad():
-        for precision in ('bf16', 'fp8'):
+        for precision in (None, 'fp8'):
             layer(x, precision=precision)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            results = [layer(x, precision=p) for p in ('bf16', 'fp8')]
+            results = [layer(x, precision=p) for p in (None, 'fp8')]
         for scale in (1.0, -1.0):
             x.copy_(torch.randn(40, 128, device='cuda', generator=gen) * scale)
             graph.replay()
             assert torch.equal(results[0], layer(x)) and torch.equal(results[1], layer(x, precision='fp8'))
     check_gemm_errors()
+
+
+def test_captured_training_step():
+    """Forward, backward and clipping in one graph, equal to the eager step bit for bit."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from msccl.ops import check_gemm_errors
+from msccl.parallel import FlatGradients, GroupedMoE
+layer = GroupedMoE(128, 96, 4, 2, std=0.1)
+flat = FlatGradients(layer.parameters(), lambda n, d: torch.empty(n, dtype=d, device='cuda'))
+x = torch.randn(60, 128, device='cuda').bfloat16()
+def step():
+    flat.zero()
+    layer(x).float().square().sum().backward()
+    return flat.clip_grad_norm(1.0)
+side = torch.cuda.Stream()
+side.wait_stream(torch.cuda.current_stream())
+with torch.cuda.stream(side):
+    step()
+torch.cuda.current_stream().wait_stream(side)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    norm = step()
+for _ in range(2):
+    x.copy_(torch.randn(60, 128, device='cuda'))
+    graph.replay()
+    got = [p.grad.clone() for p in layer.parameters()], float(norm)
+    want_norm = float(step())
+    want = [p.grad.clone() for p in layer.parameters()]
+    assert all(torch.equal(a, b) for a, b in zip(got[0], want)) and got[1] == want_norm
+check_gemm_errors()
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, '-c', code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stdout + done.stderr
