@@ -12,8 +12,7 @@
 // a sum of 2^30 elements loses nothing.  A group whose fp32 sum leaves [2^-80, 2^120] (tiny, huge, infinite or NaN values; a group
 // of zeros too) is added again in fp64, where no square of an fp32 number over- or underflows.
 //
-// Both launches are bound by HBM.  The scale kernel walks the chunks backwards: what the norm read last is still in the 126 MB
-// L2.
+// Both launches are bound by HBM.  (Walking the chunks backwards in the second, for what the norm left in L2, gains nothing.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -29,8 +28,10 @@ namespace sm100 {
 namespace {
 
 constexpr int kGradThreads = 256;
-constexpr int kGradCtasPerSm = 8;
-constexpr int kGradMaxCtas = 2048;              // partial sums of one launch
+// CTAs per SM.  256 Mi bf16 elements: the norm takes 99 us with 8 and 85 (6.3 TB/s) with 6, scaling into fp32 270 us (6.0 TB/s) with 8
+// and 285 with 6.
+constexpr int kNormCtas = 6, kScaleCtas = 8;
+constexpr int kGradMaxCtas = 2048;
 constexpr int kChunk = 16384;                   // elements
 constexpr int kFewTensors = 100;                // this list fits the 4 KB of arguments that every launch may carry
 
@@ -150,9 +151,9 @@ __global__ void __launch_bounds__(kGradThreads) grad_sum_kernel(const double* __
 template <typename S, typename D>
 __device__ __forceinline__ void chunk_scale(const S* src, D* dst, int n, float factor) {
   // The wider of the two types moves 16 bytes per lane, so that every access of a warp is one stretch of memory (8 elements a lane
-  // would write fp32 as two halves of a 32-byte sector at different times: 256 Mi bf16 -> fp32 356 us, now 269).  Element by
+  // would write fp32 as two halves of a 32-byte sector at different times: 256 Mi bf16 -> fp32 356 us, now 270).  Element by
   // element where the two sides cannot be aligned together.
-  constexpr int N = 16 / (sizeof(S) > sizeof(D) ? sizeof(S) : sizeof(D)), U = 4;
+  constexpr int N = 16 / (sizeof(S) > sizeof(D) ? sizeof(S) : sizeof(D)), U = 8;
   constexpr uintptr_t as = sizeof(S) * N, ad = sizeof(D) * N;
   int head = static_cast<int>((as - reinterpret_cast<uintptr_t>(src) % as) % as / sizeof(S));
   if (reinterpret_cast<uintptr_t>(dst + head) % ad != 0) head = n;
@@ -200,7 +201,7 @@ grad_scale_kernel(const __grid_constant__ GradList<MAX> list, const double* __re
   if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out != nullptr) *norm_out = static_cast<float>(norm);
   const double ratio = max_norm / (norm + 1e-6);
   const float factor = ratio > 1.0 ? 1.0f : static_cast<float>(ratio);        // a NaN stays one
-  for (int c = list.chunks - 1 - static_cast<int>(blockIdx.x); c >= 0; c -= gridDim.x) {
+  for (int c = blockIdx.x; c < list.chunks; c += gridDim.x) {
     const GradTensor& t = list.t[find_tensor(list, c)];
     if (factor == 1.0f && t.src == t.dst) continue;
     const long long lo = static_cast<long long>(c - t.first_chunk) * kChunk;
@@ -235,10 +236,10 @@ bool list_ok(const GradTensor* tensors, int count) {
   return chunks < (1ll << 30);
 }
 
-int grad_grid(const GradTensor* tensors, int count) {
+int grad_grid(const GradTensor* tensors, int count, int per_sm) {
   long long chunks = 0;
   for (int i = 0; i < count; ++i) chunks += (tensors[i].numel + kChunk - 1) / kChunk;
-  long long g = sm_count() * kGradCtasPerSm;
+  long long g = sm_count() * per_sm;
   if (g > kGradMaxCtas) g = kGradMaxCtas;
   return static_cast<int>(g < chunks ? g : chunks);
 }
@@ -246,11 +247,11 @@ int grad_grid(const GradTensor* tensors, int count) {
 }  // namespace
 
 // Partial sums that a launch for this list writes: one for each of its CTAs.
-int grad_norm_partials(const GradTensor* tensors, int count) { return list_ok(tensors, count) ? grad_grid(tensors, count) : 0; }
+int grad_norm_partials(const GradTensor* tensors, int count) { return list_ok(tensors, count) ? grad_grid(tensors, count, kNormCtas) : 0; }
 
 cudaError_t launch_grad_norm(const GradTensor* tensors, int count, double* partials, cudaStream_t stream) {
   if (!list_ok(tensors, count)) return cudaErrorInvalidValue;
-  const int grid = grad_grid(tensors, count);
+  const int grid = grad_grid(tensors, count, kNormCtas);
   if (count <= kFewTensors) grad_norm_kernel<kFewTensors><<<grid, kGradThreads, 0, stream>>>(make_list<kFewTensors>(tensors, count), partials);
   else grad_norm_kernel<kGradTensorsPerLaunch><<<grid, kGradThreads, 0, stream>>>(make_list<kGradTensorsPerLaunch>(tensors, count), partials);
   return cudaGetLastError();
@@ -265,7 +266,7 @@ cudaError_t launch_grad_sum(const double* partials, int count, double* sum, floa
 cudaError_t launch_grad_scale(const GradTensor* tensors, int count, const double* partials, int partial_count, double max_norm, float* norm,
                               cudaStream_t stream) {
   if (!list_ok(tensors, count) || partial_count < 1) return cudaErrorInvalidValue;
-  const int grid = grad_grid(tensors, count);
+  const int grid = grad_grid(tensors, count, kScaleCtas);
   if (count <= kFewTensors)
     grad_scale_kernel<kFewTensors><<<grid, kGradThreads, 0, stream>>>(make_list<kFewTensors>(tensors, count), partials, partial_count,
                                                                            max_norm, norm);
