@@ -11,7 +11,7 @@
 // and half of the columns each.
 //
 // What bounds it: an exchange between the roles (commit, wait, arrival) costs some hundred clocks whatever it hands over, so two or
-// four blocks of K share one (8192 x 4096 x 14336: 625 us with one, 448 with two); the operands of a 128 x 128 tile come from L2 at 19
+// four blocks of K share one (8192 x 4096 x 14336: 625 us with one, 438 with two); the operands of a 128 x 128 tile come from L2 at 19
 // TB/s, which alone takes 405 us there.  Tried: 128 x 256 tiles (128 sums a thread spill, and a spilled value comes back from L2:
 // 614 us), CTA pairs with 256 x 256 (481: one block per accumulator) and 256 x 128 tiles (438, and 549 against 519 us at 8192 x 14336 x
 // 4096).
@@ -66,10 +66,8 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void load_part(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
-__device__ __forceinline__ void load_part(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
-__device__ __forceinline__ void wait_part(uint32_t (&r)[32]) { wait_loaded(r); }
-__device__ __forceinline__ void wait_part(uint32_t (&r)[16]) {
+// Wait for this thread's tensor-memory loads; the registers pass through (as in wait_loaded).
+__device__ __forceinline__ void wait_loaded16(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
                  "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
@@ -77,7 +75,8 @@ __device__ __forceinline__ void wait_part(uint32_t (&r)[16]) {
 }
 
 // The scales of one row and one 128-column block of the result, U blocks of K at a time: while U are used, the next U are on their way
-// from L2, and they are multiplied when their turn comes.  (One block ahead, every block took as long as a load.)
+// from L2, and they are multiplied when their turn comes.  The kernel takes two exchanges' worth at a time: one block ahead, every
+// block took as long as a load; one exchange ahead, 128 x 4096 x 14336 took 39 us instead of 31.
 template <int U>
 struct ScaleStream {
   const float *sa, *sb;
@@ -201,6 +200,7 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_
       ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
       : "memory");
 }
+
 template <int BN, int AR>
 __global__ void __launch_bounds__(kFThreads, 1)
 fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const FArgs g) {
@@ -339,44 +339,44 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         scales.advance();
 #pragma unroll
         for (int turn = 0; turn < 2; ++turn) {
-        const int kb = kb0 + turn * U;
-        if (kb >= k_blocks) break;
-        ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag);
-        ok = __all_sync(kFullMask, ok);
-        if (!ok) {
-          if (lane == 0) gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 2, acc);
-          break;
-        }
-        tc_fence_after_sync();
-        const int here = min(U, k_blocks - kb);
-        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * U * BN + half * COLS);
-        auto release = [&] {
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[acc]);
-        };
-        if (left > 0) {
-          // CHUNK columns of a block at a time; the next ones are on their way while these are added, and the accumulator is free
-          // again before the last ones are
-          constexpr int PER = COLS / CHUNK;
-          uint32_t r[2][CHUNK];
-          load_part(taddr, r[0]);
-#pragma unroll
-          for (int q = 0; q < U * PER; ++q) {
-            if (q / PER >= here) break;
-            wait_part(r[q % 2]);
-            if ((q + 1) % PER != 0 || (q + 1) / PER < here)
-              load_part(taddr + (q + 1) / PER * BN + (q + 1) % PER * CHUNK, r[(q + 1) % 2]);
-            else
-              release();
-            const float2 s2 = make_float2(scales.now[turn * U + q / PER], scales.now[turn * U + q / PER]);
-#pragma unroll
-            for (int i = 0; i < CHUNK / 2; ++i) fma2(sum[q % PER * (CHUNK / 2) + i], s2, r[q % 2][2 * i], r[q % 2][2 * i + 1]);
+          const int kb = kb0 + turn * U;
+          if (kb >= k_blocks) break;
+          ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag);
+          ok = __all_sync(kFullMask, ok);
+          if (!ok) {
+            if (lane == 0) gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 2, acc);
+            break;
           }
-        } else {
-          release();
-        }
-        if (++acc == ACCS) { acc = 0; acc_phase ^= 1; }
+          tc_fence_after_sync();
+          const int here = min(U, k_blocks - kb);
+          const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * U * BN + half * COLS);
+          auto release = [&] {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[acc]);
+          };
+          if (left > 0) {
+            // CHUNK columns of a block at a time; the next ones are on their way while these are added, and the accumulator is free
+            // again before the last ones are
+            constexpr int PER = COLS / CHUNK;
+            uint32_t r[2][CHUNK];
+            tmem_ld16(taddr, r[0]);
+#pragma unroll
+            for (int q = 0; q < U * PER; ++q) {
+              if (q / PER >= here) break;
+              wait_loaded16(r[q % 2]);
+              if ((q + 1) % PER != 0 || (q + 1) / PER < here)
+                tmem_ld16(taddr + (q + 1) / PER * BN + (q + 1) % PER * CHUNK, r[(q + 1) % 2]);
+              else
+                release();
+              const float2 s2 = make_float2(scales.now[turn * U + q / PER], scales.now[turn * U + q / PER]);
+#pragma unroll
+              for (int i = 0; i < CHUNK / 2; ++i) fma2(sum[q % PER * (CHUNK / 2) + i], s2, r[q % 2][2 * i], r[q % 2][2 * i + 1]);
+            }
+          } else {
+            release();
+          }
+          if (++acc == ACCS) { acc = 0; acc_phase ^= 1; }
         }
       }
       if (ok && left > 0) store_rows(g, row - lane, left, column, sum);
@@ -417,7 +417,7 @@ cudaError_t launch(const CUtensorMap& map_a, const CUtensorMap& map_w, const FAr
 cudaError_t launch_fp8_block_gemm(const void* a, long long lda, const float* sa, long long sa_row, long long sa_block, const void* w,
                                   long long ldw, long long lde, const float* sb, const int* offsets, void* out, long long ldo, int rows,
                                   int groups, int n, int k, int bn, bool few_rows, bool zero_rest, int* error_words, cudaStream_t stream) {
-  if (rows < 1 || groups < 1 || groups > kMaxGroups || n < 8 || k < 16 || n % 8 != 0 || k % 16 != 0 || lda % 16 != 0 || ldw % 16 != 0 ||
+  if (rows < 1 || rows > kMaxRows || groups < 1 || groups > kMaxGroups || n < 8 || n > kMaxRows || k < 16 || k > kMaxRows || n % 8 != 0 || k % 16 != 0 || lda % 16 != 0 || ldw % 16 != 0 ||
       lde % 16 != 0 || ldo % 8 != 0 || (offsets == nullptr && groups != 1) || (few_rows && rows > 32))
     return cudaErrorInvalidValue;
   FArgs g;

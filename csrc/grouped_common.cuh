@@ -13,6 +13,7 @@ namespace msccl {
 namespace sm100 {
 
 constexpr int kMaxGroups = 512;
+constexpr int kMaxRows = 1 << 30;                // also of n and k: index arithmetic of tiles stays in 32 bits
 constexpr unsigned int kFullMask = 0xffffffffu;
 
 // Rows of every group and the number of tiles before it.  Offsets come from the device and may be anything: they are clamped to

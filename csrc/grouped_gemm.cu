@@ -31,7 +31,7 @@ namespace sm100 {
 namespace {
 
 constexpr int kGroupTileRows = 2048;             // rows that a group of tiles walks together (L2, see tile_coords)
-constexpr int kGEpilogueWarps = 8;               // two on each quarter of the lanes; with four the transposition of a tile took 4.8 us
+constexpr int kGEpilogueWarps = 8;               // two on each quarter of the lanes
 constexpr int kGThreads = 64 + 32 * kGEpilogueWarps;
 constexpr int kGABytes = BM * BK * 2;            // this CTA's 128 features: 16 KB
 constexpr int kGSmemLimit = 220 * 1024;
@@ -244,7 +244,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 }
 
 template <int BN, bool MN_MAJOR, bool BF16>
-cudaError_t launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const CUtensorMap& map_piece, const GroupedArgs& g, int most_tiles, cudaStream_t stream) {
+cudaError_t launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const CUtensorMap& map_piece, const GroupedArgs& g, int most_tiles,
+                   cudaStream_t stream) {
   static int cached[64] = {};
   auto kernel = grouped_gemm_kernel<BN, MN_MAJOR, BF16>;
   int dev = 0;
@@ -263,10 +264,10 @@ cudaError_t launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const CUt
 }
 
 template <int BN>
-cudaError_t launch_by_type(bool mn_major, bool bf16, const CUtensorMap& map_w, const CUtensorMap& map_x, const CUtensorMap& map_piece, const GroupedArgs& g, int most_tiles,
-                           cudaStream_t stream) {
-  if (mn_major) return bf16 ? launch<BN, true, true>(map_w, map_x, map_piece, g, most_tiles, stream) : launch<BN, true, false>(map_w, map_x, map_piece, g, most_tiles, stream);
-  return bf16 ? launch<BN, false, true>(map_w, map_x, map_piece, g, most_tiles, stream) : launch<BN, false, false>(map_w, map_x, map_piece, g, most_tiles, stream);
+cudaError_t launch_by_type(bool mn_major, bool bf16, const CUtensorMap& map_w, const CUtensorMap& map_x, const CUtensorMap& map_piece,
+                           const GroupedArgs& g, int most_tiles, cudaStream_t stream) {
+  auto run = mn_major ? (bf16 ? launch<BN, true, true> : launch<BN, true, false>) : (bf16 ? launch<BN, false, true> : launch<BN, false, false>);
+  return run(map_w, map_x, map_piece, g, most_tiles, stream);
 }
 
 }  // namespace
@@ -276,7 +277,7 @@ cudaError_t launch_by_type(bool mn_major, bool bf16, const CUtensorMap& map_w, c
 cudaError_t launch_grouped_gemm(const void* x, long long ldx, const void* w, long long ldw, long long lde, const int* offsets, void* out,
                                 long long ldo, int rows, int groups, int n, int k, bool backward, int elem, int bn, bool zero_rest,
                                 int* error_words, cudaStream_t stream) {
-  if (rows < 1 || groups < 1 || groups > kMaxGroups || n < 8 || k < 8 || n % 8 != 0 || k % 8 != 0 || ldx % 8 != 0 || ldw % 8 != 0 ||
+  if (rows < 1 || rows > kMaxRows || groups < 1 || groups > kMaxGroups || n < 8 || n > kMaxRows || k < 8 || k > kMaxRows || n % 8 != 0 || k % 8 != 0 || ldx % 8 != 0 || ldw % 8 != 0 ||
       lde % 8 != 0 || ldo % 8 != 0 || (elem != kElemBF16 && elem != kElemF16))
     return cudaErrorInvalidValue;
   GroupedArgs g;

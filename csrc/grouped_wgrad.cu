@@ -317,7 +317,7 @@ cudaError_t launch(const CUtensorMap& map_dy, const CUtensorMap& map_x, const Wg
 cudaError_t launch_grouped_wgrad(const void* dy, long long lddy, const void* x, long long ldx, const int* offsets, void* out, long long ldo,
                                  long long lde, int rows, int groups, int n, int k, int elem, bool f32_out, int* error_words,
                                  cudaStream_t stream) {
-  if (rows < 1 || groups < 1 || groups > kMaxGroups || n < 8 || k < 8 || n % 8 != 0 || k % 8 != 0 || lddy % 8 != 0 || ldx % 8 != 0 ||
+  if (rows < 1 || rows > kMaxRows || groups < 1 || groups > kMaxGroups || n < 8 || n > kMaxRows || k < 8 || k > kMaxRows || n % 8 != 0 || k % 8 != 0 || lddy % 8 != 0 || ldx % 8 != 0 ||
       ldo % (f32_out ? 4 : 8) != 0 || lde % (f32_out ? 4 : 8) != 0 || (elem != kElemBF16 && elem != kElemF16))
     return cudaErrorInvalidValue;
   WgradArgs g;
@@ -338,8 +338,8 @@ cudaError_t launch_grouped_wgrad(const void* dy, long long lddy, const void* x, 
   const long long tiles = static_cast<long long>(groups) * ((n + kWTile - 1) / kWTile) * ((k + kWTile - 1) / kWTile);
   if (tiles > (1ll << 30)) return cudaErrorInvalidValue;
   const bool bf16 = elem == kElemBF16;
-  if (f32_out) return bf16 ? launch<true, true>(map_dy, map_x, g, static_cast<int>(tiles), stream) : launch<false, true>(map_dy, map_x, g, static_cast<int>(tiles), stream);
-  return bf16 ? launch<true, false>(map_dy, map_x, g, static_cast<int>(tiles), stream) : launch<false, false>(map_dy, map_x, g, static_cast<int>(tiles), stream);
+  auto run = f32_out ? (bf16 ? launch<true, true> : launch<false, true>) : (bf16 ? launch<true, false> : launch<false, false>);
+  return run(map_dy, map_x, g, static_cast<int>(tiles), stream);
 }
 
 }  // namespace sm100

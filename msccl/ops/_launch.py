@@ -20,6 +20,7 @@ def _elsewhere(index, stream):
                 yield
 
 
+MAX_ROWS = 1 << 30                                      # kMaxRows of csrc/grouped_common.cuh
 _HERE = contextlib.nullcontext()
 # the public torch.cuda.current_device() and current_stream().cuda_stream give the same numbers in five microseconds more
 _current_device = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.current_device
@@ -70,6 +71,11 @@ def check_matrix(t, name, dtypes, unit, dims=2):
             inner = stride[d] * shape[d]
     if t.data_ptr() % 16:
         raise ValueError(f'{name} must start on a 16-byte boundary')
+
+
+def check_sizes(*sizes):
+    if max(sizes) > MAX_ROWS:
+        raise ValueError(f'rows and dimensions of a product are limited to {MAX_ROWS} (got {max(sizes)})')
 
 
 def check_offsets(offsets, experts):

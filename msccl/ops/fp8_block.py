@@ -11,8 +11,8 @@ fp32 numbers, the form in which block-quantised checkpoints come.  There are no 
 """
 import torch
 
-from msccl.ops._launch import (ELEMS, check, check_apart, check_devices, check_matrix, check_offsets, error_words, matrix_stride, on_stream,
-                               pitch, stream_handle)
+from msccl.ops._launch import (ELEMS, check, check_apart, check_devices, check_matrix, check_offsets, check_sizes, error_words, matrix_stride,
+                               on_stream, pitch, stream_handle)
 from msccl.ops.moe_rows import MAX_EXPERTS
 from msccl.runtime.native import load
 
@@ -84,6 +84,7 @@ def _check(a, sa, w, sw, offsets, out, dims):
     check_matrix(a, 'a', (_E4M3,), 16)
     if a.shape[1] != k:
         raise ValueError(f'inner dimensions differ (a {a.shape[1]}, w {k})')
+    check_sizes(a.shape[0], n, k)
     if sa.dtype != torch.float32 or sa.shape != (a.shape[0], _blocks(k)):
         raise ValueError(f'the scales of a must be float32 [{a.shape[0]}, {_blocks(k)}] (got {sa.dtype} {list(sa.shape)})')
     want = (*w.shape[:-2], _blocks(n), _blocks(k))

@@ -3,13 +3,14 @@ matrix, as ``sort_copies`` gives them) times that expert's weights, forward and 
 ``csrc/grouped_wgrad.cu``).  Any number of rows per expert, none included; there is no capacity and no padding.
 
 ``offsets`` [experts + 1] int32 stays on the device: no call waits for it.  Values are clamped to the rows and to their running
-maximum.  Rows that belong to no expert come out as zeros, or, in an ``out`` that the caller gives, are left as they were.
+maximum.  Rows that belong to no expert come out as zeros, or, in an ``out`` that the caller gives, are left as they were.  ``out`` may not
+reach into the stretch of memory between an input's first and last element.
 """
 import torch
 from torch.autograd.function import once_differentiable
 
-from msccl.ops._launch import (ELEMS, check, check_apart, check_devices, check_matrix, check_offsets, error_words, matrix_stride, on_stream,
-                               pitch, stream_handle)
+from msccl.ops._launch import (ELEMS, check, check_apart, check_devices, check_matrix, check_offsets, check_sizes, error_words, matrix_stride,
+                               on_stream, pitch, stream_handle)
 from msccl.ops.moe_rows import MAX_EXPERTS, _kernel_rows
 from msccl.runtime.native import load
 
@@ -81,6 +82,7 @@ def _check_product(x, name, w, offsets, out, backward):
     check_matrix(x, name, (w.dtype,), 8)
     if x.shape[1] != width:
         raise ValueError(f'{name} has {x.shape[1]} columns, the weights expect {width}')
+    check_sizes(x.shape[0], n, k)
     check_offsets(offsets, experts)
     if out is not None:
         check_matrix(out, 'out', (w.dtype,), 8)
@@ -113,6 +115,7 @@ def grouped_gemm_wgrad(dy, x, offsets, out=None, dtype=None, stream=None):
     check_matrix(x, 'x', _TYPES, 8)
     check_matrix(dy, 'dy', (x.dtype,), 8)
     check(x.shape[0] == dy.shape[0], f'dy has {dy.shape[0]} rows, x {x.shape[0]}')
+    check_sizes(x.shape[0], x.shape[1], dy.shape[1])
     experts = offsets.numel() - 1
     _check_experts(experts)
     check_offsets(offsets, experts)

@@ -62,6 +62,15 @@ def test_grouped_gemm_results_and_gradients():
     _refused(lambda: grouped_gemm_wgrad(_z(5, 8), x, OFFSETS), 'CUDA')
 
 
+def test_sizes_beyond_the_index_arithmetic():
+    rows = (1 << 30) + 8
+    x = torch.empty(rows, 16, dtype=BF16, device='meta')
+    _refused(lambda: grouped_gemm(x, _z(3, 8, 16), OFFSETS), 'limited')
+    _refused(lambda: grouped_gemm_wgrad(x, x, OFFSETS), 'limited')
+    a = torch.empty(rows, 16, dtype=F8, device='meta')
+    _refused(lambda: gemm_fp8_block(a, torch.zeros(rows, 1, device='meta'), _z(8, 16, dtype=F8), torch.zeros(1, 1)), 'limited')
+
+
 def _order(tokens, topk):
     return CopyOrder(torch.zeros(tokens * topk, dtype=torch.int32), torch.zeros(5, dtype=torch.int32), torch.zeros(tokens, topk, dtype=torch.int32))
 

@@ -251,6 +251,59 @@ assert not failed, failed
     assert done.returncode == 0, done.stdout + done.stderr
 
 
+def test_first_call_inside_a_capture_is_refused():
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from msccl.ops.grouped import grouped_gemm
+x, w = torch.randn(8, 64, device='cuda').bfloat16(), torch.randn(1, 64, 64, device='cuda').bfloat16()
+offsets = torch.tensor([0, 8], dtype=torch.int32, device='cuda')
+try:
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        grouped_gemm(x, w, offsets)
+except RuntimeError as e:
+    assert 'before capturing' in str(e), e
+else:
+    raise SystemExit('not refused')
+grouped_gemm(x, w, offsets)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = grouped_gemm(x, w, offsets)
+graph.replay()
+assert torch.equal(y, grouped_gemm(x, w, offsets))
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, '-c', code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stdout + done.stderr
+
+
+def test_kernels_skip_after_a_reported_timeout():
+    """The error words as a kernel that gave up leaves them: later launches return at once, the check reports and clears."""
+    from msccl.ops import GemmKernelError, check_gemm_errors
+    from msccl.ops.fp8_block import gemm_fp8_block, quantize_fp8_block, quantize_fp8_block_weight
+    from msccl.ops.gemm import _errors
+    from msccl.ops.grouped import grouped_gemm, grouped_gemm_dgrad, grouped_gemm_wgrad
+    gen = torch.Generator(device='cuda').manual_seed(7)
+    x, w = _whole(gen, 100, 64, dtype=torch.bfloat16), _whole(gen, 2, 64, 64, dtype=torch.bfloat16)
+    at, offsets = _offsets([30, 70], 0)
+    fp8 = (*quantize_fp8_block(x), *quantize_fp8_block_weight(w[0]))
+    calls = [(lambda out: grouped_gemm(x, w, offsets, out=out), (100, 64)), (lambda out: grouped_gemm_dgrad(x, w, offsets, out=out), (100, 64)),
+             (lambda out: grouped_gemm_wgrad(x, x, offsets, out=out), (2, 64, 64)), (lambda out: gemm_fp8_block(*fp8, out=out), (100, 64))]
+    check_gemm_errors()
+    for call, shape in calls:
+        out = torch.full(shape, 7.0, dtype=torch.bfloat16, device='cuda')
+        _errors('cuda:0')[0] = 1
+        call(out)
+        with pytest.raises(GemmKernelError):
+            check_gemm_errors()
+        assert torch.all(out == 7.0)
+        call(out)
+        check_gemm_errors()
+        assert not torch.all(out == 7.0)
+
+
 def test_far_rows():
     """Offsets of elements beyond 2^31: 150000 rows of 16384 columns."""
     from msccl.ops import check_gemm_errors
