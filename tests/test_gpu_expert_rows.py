@@ -93,6 +93,23 @@ def test_rows_and_their_gradients(tokens, topk, experts, hidden, dropped, dtype)
     assert torch.equal(torch.autograd.grad(combine_rows(ys, weights.detach(), order), ys, dy)[0], dys)
 
 
+def test_gradients_are_difference_quotients():
+    """Both operators are linear in each operand: f(a + d) - f(a) = <gradient, d>, exactly for small whole numbers in fp32."""
+    from msccl.ops.moe_rows import combine_rows, gather_rows, sort_copies
+    gen = torch.Generator(device='cuda').manual_seed(9)
+
+    def whole(*shape):
+        return torch.randint(-4, 5, shape, device='cuda', generator=gen).float()
+    order = sort_copies(_chosen(gen, 40, 3, 6, True), 6)
+    x, ys, weights, cx, cy = whole(40, 20), whole(120, 20), whole(40, 3), whole(120, 20), whole(40, 20)
+    for f, operand, c in ((lambda t: gather_rows(t, order), x, cx), (lambda t: combine_rows(t, weights, order), ys, cy),
+                          (lambda t: combine_rows(ys, t, order), weights, cy)):
+        leaf = operand.clone().requires_grad_()
+        (f(leaf) * c).sum().backward()
+        d = whole(*operand.shape)
+        assert ((f(operand + d) - f(operand)).double() * c.double()).sum() == (leaf.grad.double() * d.double()).sum()
+
+
 def test_rows_with_strides_and_expanded_gradients():
     from msccl.ops.moe_rows import combine_rows, gather_rows, sort_copies
     gen = torch.Generator(device='cuda').manual_seed(0)
