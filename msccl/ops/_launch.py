@@ -50,32 +50,50 @@ def check(condition, message):
         raise ValueError(message)
 
 
-def check_matrix(t, name, dtypes, unit, dims=2):
-    """``t`` has ``dims`` dimensions, its rows are contiguous, start on 16-byte boundaries and hold a multiple of ``unit`` elements.
-    A stride that no index uses (one row, one matrix) may have any value."""
+def check_matrix(t, name, dtypes, unit):
+    """``t`` [rows, columns]: contiguous rows of a multiple of ``unit`` elements that start on 16-byte boundaries and do not overlap.
+    Returns rows, columns and the row stride (that of a single row, which no index uses, is its length)."""
     shape, stride, dtype = t.shape, t.stride(), t.dtype
-    if dtype not in dtypes:
-        raise ValueError(f'{name} must be {" or ".join(str(d) for d in dtypes)} (got {dtype})')
-    if len(shape) != dims:
-        raise ValueError(f'{name} must have {dims} dimensions (got {len(shape)})')
-    inner = shape[-1]
-    if inner <= 0 or inner % unit:
-        raise ValueError(f'the last dimension of {name} must be a positive multiple of {unit} (got {inner})')
-    if stride[-1] != 1:
+    if dtype in dtypes and len(shape) == 2:
+        rows, columns = shape
+        pitch = stride[0] if rows > 1 else columns
+        if columns > 0 and not columns % unit and stride[1] == 1 and pitch >= columns and not (
+                pitch * dtype.itemsize % 16 or t.data_ptr() % 16):
+            return rows, columns, pitch
+    _refuse(t, name, dtypes, unit, 2)
+
+
+def check_matrices(t, name, dtypes, unit):
+    """``t`` [count, rows, columns]: ``check_matrix`` for each, and matrices that do not overlap.  Returns count, rows, columns, the row
+    stride and the matrix stride."""
+    shape, stride, dtype = t.shape, t.stride(), t.dtype
+    if dtype in dtypes and len(shape) == 3:
+        count, rows, columns = shape
+        pitch = stride[1] if rows > 1 else columns
+        between = stride[0] if count > 1 else rows * pitch
+        if columns > 0 and not columns % unit and stride[2] == 1 and pitch >= columns and between >= rows * pitch - (pitch - columns) and not (
+                pitch * dtype.itemsize % 16 or between * dtype.itemsize % 16 or t.data_ptr() % 16):
+            return count, rows, columns, pitch, between
+    _refuse(t, name, dtypes, unit, 3)
+
+
+def _refuse(t, name, dtypes, unit, dims):
+    if t.dtype not in dtypes:
+        raise ValueError(f'{name} must be {" or ".join(str(d) for d in dtypes)} (got {t.dtype})')
+    if t.dim() != dims:
+        raise ValueError(f'{name} must have {dims} dimensions (got {t.dim()})')
+    if t.shape[-1] <= 0 or t.shape[-1] % unit:
+        raise ValueError(f'the last dimension of {name} must be a positive multiple of {unit} (got {t.shape[-1]})')
+    if t.stride(-1) != 1:
         raise ValueError(f'the rows of {name} must be contiguous')
-    step = 16 // dtype.itemsize
-    for d in range(dims - 2, -1, -1):
-        if shape[d] > 1:
-            if stride[d] % step or stride[d] < inner:
-                raise ValueError(f'the strides of {name} must be multiples of 16 bytes and its rows must not overlap (stride {stride[d]})')
-            inner = stride[d] * shape[d]
     if t.data_ptr() % 16:
         raise ValueError(f'{name} must start on a 16-byte boundary')
+    raise ValueError(f'the strides of {name} must be multiples of 16 bytes and its rows must not overlap (strides {t.stride()})')
 
 
-def check_sizes(*sizes):
-    if max(sizes) > MAX_ROWS:
-        raise ValueError(f'rows and dimensions of a product are limited to {MAX_ROWS} (got {max(sizes)})')
+def check_sizes(rows, n, k):
+    if rows > MAX_ROWS or n > MAX_ROWS or k > MAX_ROWS:
+        raise ValueError(f'rows and dimensions of a product are limited to {MAX_ROWS} (got {rows}, {n}, {k})')
 
 
 def check_offsets(offsets, experts):
@@ -83,18 +101,14 @@ def check_offsets(offsets, experts):
         raise ValueError(f'offsets must be a contiguous [{experts + 1}] int32 tensor (got {list(offsets.shape)} {offsets.dtype})')
 
 
-def check_devices(**tensors):
-    """All tensors (``None`` ones apart) are on one CUDA device; returns its index."""
-    index = None
-    for name, t in tensors.items():
-        if t is not None:
-            at = t.get_device()
-            if at != index:
-                if at < 0 or not t.is_cuda:
-                    raise ValueError(f'{name} must be a CUDA tensor')
-                if index is not None:
-                    raise ValueError(f'{name} is on cuda:{at}, the other tensors on cuda:{index}')
-                index = at
+def check_devices(names, *tensors):
+    """All tensors (``None`` ones apart) are on one CUDA device; returns its index.  ``names``: theirs, for the message."""
+    index = tensors[0].get_device()
+    if index < 0 or not tensors[0].is_cuda:
+        raise ValueError(f'{names.split()[0]} must be a CUDA tensor')
+    for i, t in enumerate(tensors):
+        if t is not None and t.get_device() != index:
+            raise ValueError(f'{names.split()[i]} is on {t.device}, {names.split()[0]} on cuda:{index}')
     return index
 
 

@@ -10,9 +10,10 @@ Beside the MX format of ``msccl.ops.gemm`` (a power of two per 32 values, applie
 fp32 numbers, the form in which block-quantised checkpoints come.  There are no gradients: this is the path for serving.
 """
 import torch
+from torch.autograd.graph import increment_version
 
-from msccl.ops._launch import (ELEMS, check, check_apart, check_devices, check_matrix, check_offsets, check_sizes, error_words, matrix_stride,
-                               on_stream, pitch, stream_handle)
+from msccl.ops._launch import (ELEMS, check, check_apart, check_devices, check_matrices, check_matrix, check_offsets, check_sizes, error_words,
+                               on_stream, stream_handle)
 from msccl.ops.moe_rows import MAX_EXPERTS
 from msccl.runtime.native import load
 
@@ -24,19 +25,26 @@ def _blocks(size):
     return -(-size // BLOCK)
 
 
+def _weight(w, dtypes):
+    """Matrices, rows, columns, row stride and matrix stride of a [n, k] or [experts, n, k] weight."""
+    if w.dim() == 3:
+        return check_matrices(w, 'w', dtypes, 16)
+    n, k, pitch = check_matrix(w, 'w', dtypes, 16)
+    return 1, n, k, pitch, n * pitch
+
+
 def quantize_fp8_block(x, stream=None):
     """``x`` [rows, k] fp32, bf16 or fp16 (k a multiple of 16) -> ``(q, scales)``: e4m3 [rows, k] and float32 [rows, ceil(k / 128)].
     ``scale = max(largest magnitude, 2 ** -100) / 448`` over the block, ``q = e4m3(x / scale)``, each rounded once.  The scales
     of neighbouring rows lie next to each other in memory, as the product reads them.  A NaN or an infinity makes its block NaN
     (or zero beside an infinity)."""
-    check_matrix(x, 'x', ELEMS, 16)
-    index = check_devices(x=x)
+    rows, k, pitch = check_matrix(x, 'x', ELEMS, 16)
+    index = check_devices('x', x)
     with on_stream(index, stream, (x,)):
-        rows, k = x.shape
-        q = torch.empty(rows, k, dtype=_E4M3, device=x.device)
-        scales = torch.empty(_blocks(k), rows, dtype=torch.float32, device=x.device).t()
+        q = torch.empty((rows, k), dtype=_E4M3, device=x.device)
+        scales = torch.empty((_blocks(k), rows), dtype=torch.float32, device=x.device).t()
         if rows:
-            load().quantize_rows(x.data_ptr(), pitch(x), q.data_ptr(), scales.data_ptr(), 1, rows, rows, k, ELEMS[x.dtype], stream_handle(index))
+            load().quantize_rows(x.data_ptr(), pitch, q.data_ptr(), scales.data_ptr(), 1, rows, rows, k, ELEMS[x.dtype], stream_handle(index))
     return q, scales
 
 
@@ -44,16 +52,14 @@ def quantize_fp8_block_weight(w, stream=None):
     """``w`` [n, k] or [experts, n, k] -> e4m3 of the same shape and float32 scales [.., ceil(n / 128), ceil(k / 128)], by the rule of
     ``quantize_fp8_block`` over blocks of 128 x 128."""
     check(w.dim() in (2, 3), f'w must be [n, k] or [experts, n, k] (got {w.dim()} dimensions)')
-    check_matrix(w, 'w', ELEMS, 16, dims=w.dim())
+    experts, n, k, pitch, between = _weight(w, ELEMS)
     check(w.numel() > 0, 'w is empty')
-    index = check_devices(w=w)
-    n, k = w.shape[-2:]
-    experts = w.shape[0] if w.dim() == 3 else 1
+    index = check_devices('w', w)
     check(experts <= 65535, f'at most 65535 matrices at once (got {experts})')
     with on_stream(index, stream, (w,)):
         q = torch.empty(w.shape, dtype=_E4M3, device=w.device)
         scales = torch.empty(*w.shape[:-2], _blocks(n), _blocks(k), dtype=torch.float32, device=w.device)
-        load().quantize_blocks(w.data_ptr(), pitch(w), w.stride(0) if w.dim() == 3 else 0, q.data_ptr(), scales.data_ptr(), experts, n, k,
+        load().quantize_blocks(w.data_ptr(), pitch, between, q.data_ptr(), scales.data_ptr(), experts, n, k,
                                ELEMS[w.dtype], stream_handle(index))
     return q, scales
 
@@ -76,43 +82,41 @@ def _tile_columns(rows, groups, n):
     return 32
 
 
-def _check(a, sa, w, sw, offsets, out, dims):
-    check_matrix(w, 'w', (_E4M3,), 16, dims=dims)
-    n, k = w.shape[-2:]
+def _product(a, sa, w, sw, offsets, out, stream, dims):
+    check(w.dim() == dims, f'w must have {dims} dimensions (got {w.dim()})')
+    groups, n, k, w_pitch, w_stride = _weight(w, (_E4M3,))
     if n <= 0 or n % 8:
         raise ValueError(f'the rows of a weight must be a positive multiple of 8 (got {n})')
-    check_matrix(a, 'a', (_E4M3,), 16)
-    if a.shape[1] != k:
-        raise ValueError(f'inner dimensions differ (a {a.shape[1]}, w {k})')
-    check_sizes(a.shape[0], n, k)
-    if sa.dtype != torch.float32 or sa.shape != (a.shape[0], _blocks(k)):
-        raise ValueError(f'the scales of a must be float32 [{a.shape[0]}, {_blocks(k)}] (got {sa.dtype} {list(sa.shape)})')
-    want = (*w.shape[:-2], _blocks(n), _blocks(k))
+    rows, columns, a_pitch = check_matrix(a, 'a', (_E4M3,), 16)
+    if columns != k:
+        raise ValueError(f'inner dimensions differ (a {columns}, w {k})')
+    check_sizes(rows, n, k)
+    k_blocks = _blocks(k)
+    if sa.dtype != torch.float32 or sa.shape != (rows, k_blocks):
+        raise ValueError(f'the scales of a must be float32 [{rows}, {k_blocks}] (got {sa.dtype} {list(sa.shape)})')
+    want = (_blocks(n), k_blocks) if dims == 2 else (groups, _blocks(n), k_blocks)
     if sw.dtype != torch.float32 or sw.shape != want or not sw.is_contiguous():
         raise ValueError(f'the scales of w must be contiguous float32 {list(want)} (got {sw.dtype} {list(sw.shape)})')
     if offsets is not None:
-        check(1 <= w.shape[0] <= MAX_EXPERTS, f'between 1 and {MAX_EXPERTS} experts are supported (got {w.shape[0]})')
-        check_offsets(offsets, w.shape[0])
+        if not 1 <= groups <= MAX_EXPERTS:
+            raise ValueError(f'between 1 and {MAX_EXPERTS} experts are supported (got {groups})')
+        check_offsets(offsets, groups)
+    out_pitch = n
     if out is not None:
-        check_matrix(out, 'out', (torch.bfloat16,), 8)
-        check(out.shape == (a.shape[0], n), f'out must be [{a.shape[0]}, {n}] (got {list(out.shape)})')
+        *shape, out_pitch = check_matrix(out, 'out', (torch.bfloat16,), 8)
+        check(shape == [rows, n], f'out must be [{rows}, {n}] (got {shape})')
         check_apart(out, a=a, sa=sa, w=w, sw=sw)
-    return check_devices(a=a, sa=sa, w=w, sw=sw, offsets=offsets, out=out)
-
-
-def _product(a, sa, w, sw, offsets, out, stream, dims):
-    index = _check(a, sa, w, sw, offsets, out, dims)
+    index = check_devices('a sa w sw offsets out', a, sa, w, sw, offsets, out)
     with on_stream(index, stream, (a, sa, w, sw, offsets, out)):
-        rows, (n, k) = a.shape[0], w.shape[-2:]
-        groups = w.shape[0] if dims == 3 else 1
         zero_rest = out is None and offsets is not None
         if out is None:
-            out = torch.empty(rows, n, dtype=torch.bfloat16, device=a.device)
+            out = torch.empty((rows, n), dtype=torch.bfloat16, device=a.device)
+        else:
+            increment_version(out)
         if rows:
-            load().fp8_block_gemm(a.data_ptr(), pitch(a), sa.data_ptr(), *sa.stride(), w.data_ptr(), pitch(w),
-                                  matrix_stride(w) if dims == 3 else n * pitch(w), sw.data_ptr(), 0 if offsets is None else offsets.data_ptr(),
-                                  out.data_ptr(), pitch(out), rows, groups, n, k, _tile_columns(rows, groups, n), rows <= 32, zero_rest,
-                                  error_words(index), stream_handle(index))
+            load().fp8_block_gemm(a.data_ptr(), a_pitch, sa.data_ptr(), *sa.stride(), w.data_ptr(), w_pitch, w_stride, sw.data_ptr(),
+                                  0 if offsets is None else offsets.data_ptr(), out.data_ptr(), out_pitch, rows, groups, n, k,
+                                  _tile_columns(rows, groups, n), rows <= 32, zero_rest, error_words(index), stream_handle(index))
     return out
 
 

@@ -38,11 +38,11 @@ def sort_copies(experts, num_experts, stream=None):
         raise ValueError(f'sort_copies needs at least one token, k <= {MAX_TOPK} and at most {MAX_COPIES} copies (got {tokens} x {topk})')
     if not 1 <= num_experts <= MAX_EXPERTS:
         raise ValueError(f'num_experts must be within 1 and {MAX_EXPERTS} (got {num_experts})')
-    index = check_devices(experts=experts)
+    index = check_devices('experts', experts)
     with on_stream(index, stream, (experts,)):
         experts = experts.contiguous()
         native = load()
-        workspace = native.sort_copies_workspace(copies, num_experts)
+        workspace = native.sort_copies_workspace(copies, num_experts) if copies > 1024 else 0
         table = torch.empty(2 * copies + num_experts + 1, dtype=torch.int32, device=experts.device)
         sorted_copy, position, offsets = table.split((copies, copies, num_experts + 1))
         counts = torch.empty(workspace, dtype=torch.int32, device=experts.device).data_ptr() if workspace else 0
@@ -129,7 +129,7 @@ def gather_rows(x, order, stream=None):
     tokens = order.position.shape[0]
     if x.shape[0] != tokens:
         raise ValueError(f'x has {x.shape[0]} rows, the order {tokens} tokens')
-    with on_stream(check_devices(x=x, order=order.position), stream, (x, order.position)):
+    with on_stream(check_devices('x order', x, order.position), stream, (x, order.position)):
         return _Gather.apply(x, order) if torch.is_grad_enabled() and x.requires_grad else _scatter(x, order)
 
 
@@ -143,7 +143,7 @@ def combine_rows(ys, weights, order, stream=None):
         raise ValueError(f'ys has {ys.shape[0]} rows, the order {tokens * topk} copies')
     if weights.dtype != torch.float32 or weights.shape != (tokens, topk):
         raise ValueError(f'weights must be a [{tokens}, {topk}] float32 tensor')
-    with on_stream(check_devices(ys=ys, weights=weights, order=order.position), stream, (ys, weights, order.position)):
+    with on_stream(check_devices('ys weights order', ys, weights, order.position), stream, (ys, weights, order.position)):
         weights = weights.contiguous()
         needs = torch.is_grad_enabled() and (ys.requires_grad or weights.requires_grad)
         return _Combine.apply(ys, weights, order) if needs else _combine(ys, weights, order)
