@@ -7,9 +7,11 @@
 // the device only: every CTA derives the same list of tiles from the offsets, so nothing is copied to the host.
 //
 // The weights are the M operand and the rows of the group the N operand of the MMA: 256 features (of a CTA pair, cta_group::2)
-// by up to BN = 64 or 256 rows, and the last tile of a group is only as wide as its rows need, in steps of 32: N is a field of the
-// instruction.  (With tiles of 256 rows throughout, 8192 rows over 7 groups were padded by 11 %.)  Rows of a tile that belong to the
-// next group only reach columns of the accumulator that are not stored, whatever they hold.  What is left of both operands behind the reduction dimension reads as zero.
+// by up to BN = 64 or 256 rows; N is a field of the instruction, so a group of 700 rows is cut into 256 + 256 + 188 or, better, into
+// three about equal tiles, in steps of 32 rows.  8192 rows in 8 unequal groups of 14336 x 4096: 611 us, 1.58 PFLOP/s, with equal tiles,
+// 693 with full ones and a narrow last one (the pair that gets one full tile more sets the time), 825 run without a pause with full
+// ones only, 784 with equal ones (the power cap).  Rows of a tile that belong to the next group only reach columns of the accumulator
+// that are not stored, whatever they hold.  What is left of both operands behind the reduction dimension reads as zero.
 //
 // The accumulator holds a feature per lane and a row per column; the epilogue transposes it (transpose_chunk).
 //
@@ -103,14 +105,16 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   const bool skip = ld_shared_cluster_u32(map_to_cta(smem_u32(&s_skip), 0)) != 0;
   const int num_tiles = table.tile_start[g.groups];
 
-  // tile -> group e, first row, rows (a multiple of 32) and first feature; e only moves forward
+  // tile -> group e, first row, width (rows, a multiple of 32) and first feature; e only moves forward.  A group of r rows has
+  // ceil(r / BN) tiles; since all but one of them at full width would not hold it, none of them is empty at any width that holds it.
   auto locate = [&](int tile, int& e, int& row, int& width, int& feature) {
     while (tile >= table.tile_start[e + 1]) ++e;
     const int rows = table.row_start[e + 1] - table.row_start[e];
     int tm, tn;
-    tile_coords(tile - table.tile_start[e], (rows + BN - 1) / BN, f_tiles, kGroupTileRows / BN, tm, tn);
-    row = table.row_start[e] + tm * BN;
-    width = min(BN, (table.row_start[e + 1] - row + 31) / 32 * 32);
+    const int tiles = (rows + BN - 1) / BN, each = ((rows + tiles - 1) / tiles + 31) / 32 * 32;
+    tile_coords(tile - table.tile_start[e], tiles, f_tiles, kGroupTileRows / BN, tm, tn);
+    row = table.row_start[e] + tm * each;
+    width = min(each, (table.row_start[e + 1] - row + 31) / 32 * 32);
     feature = tn * 2 * BM;
   };
 
@@ -125,7 +129,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         int row, width, feature;
         locate(tile, e, row, width, feature);
         const int pieces = (width / 2 + 31) / 32;      // of this CTA's width / 2 rows
-        const uint32_t bytes = kGABytes + (width == BN ? Geo::kBBytes : pieces * Geo::kPiece);
+        const bool whole = pieces * Geo::kPiece == Geo::kBBytes;
+        const uint32_t bytes = kGABytes + pieces * Geo::kPiece;
         row += static_cast<int>(rank) * (width / 2);
         feature += static_cast<int>(rank) * BM;
         for (int kb = 0; kb < k_blocks; ++kb) {
@@ -143,7 +148,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
           } else {
             tma_pair_3d(a_dst, &map_w, bar, kb * BK, feature, e);
           }
-          if (width == BN) {
+          if (whole) {
             tma_pair_2d(a_dst + kGABytes, &map_x, bar, kb * BK, row);
           } else {
             for (int p = 0; p < pieces; ++p) tma_pair_2d(a_dst + kGABytes + p * Geo::kPiece, &map_piece, bar, kb * BK, row + 32 * p);
@@ -207,7 +212,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BN);
       const int f = feature + static_cast<int>(rank) * BM + quarter * 32 + (lane & ~7);       // this lane stores features f .. f + 7
       const bool in = f < g.features;
-      const int columns = min(BN, row_end - row);
+      const int columns = min(width, row_end - row);
       for (int c = half * 32; c < columns; c += 64) {
         uint32_t r[32];
         tmem_ld32(taddr + c, r);

@@ -21,7 +21,7 @@ _TYPES = (torch.bfloat16, torch.float16)
 def _tile_rows(rows, experts):
     """The most rows of a tile, from the mean size of a group (the sizes themselves are on the device): tiles of 64 leave room for more
     of the weights on their way, tiles of 256 read them less often.  Microseconds with 64 / 256 rows, forward: 32 rows x 8 experts of
-    14336 x 4096 164 / 178; 4096 x 64 of 1024 x 2048 72 / 72; 1024 x 8 of 4096 x 4096 80 / 72; 8192 x 8 of 14336 x 4096 1115 / 696."""
+    14336 x 4096 165 / 178; 4096 x 64 of 1024 x 2048 71 / 73; 1024 x 8 of 4096 x 4096 81 / 72; 8192 x 8 of 14336 x 4096 1097 / 611."""
     return 64 if rows <= 48 * min(rows, experts) else 256
 
 
