@@ -341,8 +341,7 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         for (int turn = 0; turn < 2; ++turn) {
           const int kb = kb0 + turn * U;
           if (kb >= k_blocks) break;
-          ok = mbar_wait(&acc_full[acc], acc_phase, abort_flag);
-          ok = __all_sync(kFullMask, ok);
+          ok = mbar_wait_warp(&acc_full[acc], acc_phase, abort_flag);
           if (!ok) {
             if (lane == 0) gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_ACC, 2, acc);
             break;

@@ -92,29 +92,10 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// mbar_wait whose first polls neither suspend the thread nor read the clock: where the wait is on the critical path of every block of
-// K, waking up is too.
-__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-  return done != 0;
-}
-__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-#pragma unroll 1
-  for (int i = 0; i < 256; ++i)
-    if (mbar_test_wait(bar, parity)) return true;
-  return mbar_wait(bar, parity, abort_flag);
-}
-
-// Wait of a whole warp: one lane polls for all.
+// Wait of a whole warp.  (All lanes poll: one lane that tells the others is later by a shuffle and a branch, which an fp8 block notices.)
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  int ok = 1;
-  if (threadIdx.x % 32 == 0) ok = mbar_wait_soon(bar, parity, abort_flag) ? 1 : 0;
-  return __shfl_sync(kFullMask, ok, 0) != 0;
+  const bool ok = mbar_wait(bar, parity, abort_flag);
+  return __all_sync(kFullMask, ok);
 }
 
 // Operand whose M (or N) dimension is the contiguous one, 128-byte swizzle: slabs of 64 elements x 64 reduction rows (8 KB, 128
