@@ -1,9 +1,12 @@
 // Gradient of the matrices of grouped products, for sm_100a:  dw[e, n, k] = sum over the rows t of group e of dy[t, n] x[t, k].
 //
 // Both operands are read as they lie in memory: the reduction runs over rows, so both are MN-major (64 features x 64 rows slabs of
-// 8 KB).  CTA pairs (cta_group::2) compute 256 x 256 tiles; a group without rows writes zeros.  x is the M operand, so that
-// the lanes of an accumulator run along k, the contiguous dimension of the result.  8 groups of 1024 rows, n = k = 4096: 162 us, 1.70
-// PFLOP/s; of a few rows each the result's 2.5 TB/s of writes are the bound (3.7 us per tile).
+// 8 KB).  CTA pairs (cta_group::2) compute 256 x 256 tiles; a group without rows writes zeros.  8 groups of 1024 rows, n = k = 4096:
+// 168 us, 1.64 PFLOP/s; of few rows the writes of the result are the bound (64 groups of 64 rows, n = k = 2048: 139 us, 3.9 TB/s).
+//
+// Stores of whole lines: in 16 bits dy is the M operand, a lane of the accumulator is a row n, and eight lanes exchange pieces so that
+// they store 128 consecutive bytes of k.  (With the lanes along k a warp has 64 bytes of a row, and the same 64 groups took 215 us.)
+// For fp32 x is the M operand: 32 lanes along k are 128 bytes without an exchange (the exchange: 8 x 1024 rows 2 % more).
 //
 // The reduction is ragged: the last 64-row block of a group also covers rows of the next group (or memory behind the last one, which
 // may hold anything).  Those rows have to be zero in both operands, since 0 times infinity is not 0.  So that block goes a way of
@@ -19,8 +22,6 @@
 // memory at cluster scope and took 0.55 us of 0.83 us per block; nothing of that kind is in the loop.
 #include <cuda.h>
 #include <cuda_runtime.h>
-
-#include <type_traits>
 
 #include "expert_ops.h"
 #include "gemm_sm100.cuh"
@@ -43,6 +44,11 @@ constexpr int kWTmemCols = 2 * kWTile;
 // the pipeline, the block on its own, row_start of the groups, the barriers: 226 KB, so the base has to be aligned as it is
 constexpr int kWTableBytes = (kMaxGroups + 1) * 4 + 12;
 constexpr size_t kWSmem = static_cast<size_t>(kWStages + 1) * kWStageBytes + kWTableBytes + 256;
+// All CTAs finish a tile of equal groups at about the same time.  Stored at once, their results hold up the loads of the next tiles for longer
+// than the pipeline lasts, so from kWPacedRows rows on, where the products leave time, the stores are spread out by a pause (in ns)
+// after every 64 values of a row, or half of it after every 32 rows of fp32.  n = k = 4096, without / with pauses: 8 x 1024 rows
+// 174 / 168 us, in fp32 213 / 205; 8 x 768 rows 139 / 139, in fp32 176 / 165; 2 x 4096 rows the same.
+constexpr int kWPacedRows = 768, kWPause = 500;
 static_assert(kWSmem <= 227 * 1024 && kWTableBytes % 16 == 0, "");
 
 struct WgradArgs {
@@ -53,9 +59,45 @@ struct WgradArgs {
   int* error_words;
 };
 
+// 64 columns of this lane's row of the accumulator as 16-bit values, in eight pieces of eight.
+template <bool BF16>
+__device__ __forceinline__ void load_row(uint32_t taddr, uint4 (&v)[8]) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint32_t r[32];
+    tmem_ld32(taddr + 32 * half, r);
+    wait_loaded(r);
+    auto pack = [&](int i) { return pack_16bit(BF16, __uint_as_float(r[i]), __uint_as_float(r[i + 1])); };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[4 * half + i] = make_uint4(pack(8 * i), pack(8 * i + 2), pack(8 * i + 4), pack(8 * i + 6));
+  }
+}
+
+// From piece i of the lane's own row to piece lane % 8 of row i of its eight lanes, which then store 128 consecutive bytes together.
+// An exchange for each bit that lane and piece swap, 48 shuffles.
+__device__ __forceinline__ void transpose_lines(uint4 (&v)[8], int lane) {
+#pragma unroll
+  for (int bit = 1; bit < 8; bit *= 2) {
+    const bool up = (lane & bit) != 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i & bit) continue;
+      uint4 &low = v[i], &high = v[i | bit];
+      const uint4 give = up ? low : high;
+      uint4 got;
+      got.x = __shfl_xor_sync(kFullMask, give.x, bit);
+      got.y = __shfl_xor_sync(kFullMask, give.y, bit);
+      got.z = __shfl_xor_sync(kFullMask, give.z, bit);
+      got.w = __shfl_xor_sync(kFullMask, give.w, bit);
+      if (up) low = got;
+      else high = got;
+    }
+  }
+}
+
 template <bool BF16, bool F32OUT>
 __global__ void __launch_bounds__(kWThreads, 1)
-grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_x, const WgradArgs g) {
+grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const WgradArgs g) {
   constexpr int S = kWStages;
   extern __shared__ __align__(1024) uint8_t stage_base[];
   uint8_t* tail_base = stage_base + static_cast<size_t>(S) * kWStageBytes;
@@ -94,8 +136,8 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
       gemm_fail(g.error_words, abort_flag, GEMM_TIMEOUT_EMPTY, 9, 0);
     }
     mbar_fence_init();
-    prefetch_tensormap(&map_dy);
-    prefetch_tensormap(&map_x);
+    prefetch_tensormap(&map_a);
+    prefetch_tensormap(&map_b);
   }
   if (warp == 1) tmem_alloc_pair(tmem_slot, kWTmemCols);
   if (warp == 2) build_row_starts(row_start, g.offsets, g.groups, g.rows);
@@ -123,8 +165,7 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
       for (int tile = first; tile < num_tiles && ok; tile += step) {
         int e, n0, k0;
         locate(tile, e, n0, k0);
-        n0 += static_cast<int>(rank) * BM;
-        k0 += static_cast<int>(rank) * BM;
+        const int a0 = (F32OUT ? k0 : n0) + static_cast<int>(rank) * BM, b0 = (F32OUT ? n0 : k0) + static_cast<int>(rank) * BM;
         const int lo = row_start[e], end = row_start[e + 1];
         for (int r = lo; r + BK <= end; r += BK) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) {
@@ -135,10 +176,10 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
           uint8_t* dst = stage_base + static_cast<size_t>(stage) * kWStageBytes;
           const uint32_t bar = map_to_cta(smem_u32(&full_bar[stage]), 0);
           if (leader) mbar_expect_tx(&full_bar[stage], 2 * kWStageBytes);
-          tma_pair_2d(dst, &map_x, bar, k0, r);
-          tma_pair_2d(dst + kSlabBytes, &map_x, bar, k0 + 64, r);
-          tma_pair_2d(dst + kWOperand, &map_dy, bar, n0, r);
-          tma_pair_2d(dst + kWOperand + kSlabBytes, &map_dy, bar, n0 + 64, r);
+          tma_pair_2d(dst, &map_a, bar, a0, r);
+          tma_pair_2d(dst + kSlabBytes, &map_a, bar, a0 + 64, r);
+          tma_pair_2d(dst + kWOperand, &map_b, bar, b0, r);
+          tma_pair_2d(dst + kWOperand + kSlabBytes, &map_b, bar, b0 + 64, r);
           if (++stage == S) { stage = 0; phase ^= 1; }
         }
       }
@@ -195,18 +236,17 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
     for (int tile = first; tile < num_tiles; tile += step) {
       int e, n0, k0;
       locate(tile, e, n0, k0);
-      n0 += static_cast<int>(rank) * BM;
-      k0 += static_cast<int>(rank) * BM;
+      const int a0 = (F32OUT ? k0 : n0) + static_cast<int>(rank) * BM, b0 = (F32OUT ? n0 : k0) + static_cast<int>(rank) * BM;
       const int left = (row_start[e + 1] - row_start[e]) % BK, r0 = row_start[e + 1] - left;
       if (left == 0) continue;
       bool ok = mbar_wait_warp(tail_empty, phase ^ 1, abort_flag);
       if (ok) {
         if (elect_one()) {
           mbar_expect_tx(tail_full, kWStageBytes);
-          tma_load_2d(tail_base, &map_x, tail_full, k0, r0);
-          tma_load_2d(tail_base + kSlabBytes, &map_x, tail_full, k0 + 64, r0);
-          tma_load_2d(tail_base + kWOperand, &map_dy, tail_full, n0, r0);
-          tma_load_2d(tail_base + kWOperand + kSlabBytes, &map_dy, tail_full, n0 + 64, r0);
+          tma_load_2d(tail_base, &map_a, tail_full, a0, r0);
+          tma_load_2d(tail_base + kSlabBytes, &map_a, tail_full, a0 + 64, r0);
+          tma_load_2d(tail_base + kWOperand, &map_b, tail_full, b0, r0);
+          tma_load_2d(tail_base + kWOperand + kSlabBytes, &map_b, tail_full, b0 + 64, r0);
         }
         __syncwarp();
         ok = mbar_wait_warp(tail_full, phase, abort_flag);
@@ -243,37 +283,49 @@ grouped_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_co
         tc_fence_after_sync();
       }
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * kWTile);
-      const int columns = min(kWTile, g.n - n0);
-      // fp32: a lane stores value k of row n0 + c + i; 16 bits: values k .. k + 7 of row n0 + c + 8 m + lane % 8
-      const int k = k0 + static_cast<int>(rank) * BM + quarter * 32 + (F32OUT ? lane : lane & ~7), lane_row = F32OUT ? 0 : lane & 7;
-      const bool in = k < g.k;
-      using Out = std::conditional_t<F32OUT, float, uint16_t>;
-      Out* dst = static_cast<Out*>(g.out) + e * g.lde + (n0 + lane_row) * g.ldo + k;
-      const long long row8 = 8 * g.ldo;
-      for (int c = 0; c < columns; c += 32) {
-        uint32_t r[32];
-        if (empty) {
+      const int lanes_at = static_cast<int>(rank) * BM + quarter * 32;
+      const bool paced = row_start[e + 1] - row_start[e] >= kWPacedRows && tile + step < num_tiles;
+      if constexpr (F32OUT) {
+        // a lane stores value k of the rows n0, n0 + 1, ...
+        const int columns = min(kWTile, g.n - n0), k = k0 + lanes_at + lane;
+        float* dst = static_cast<float*>(g.out) + e * g.lde + n0 * g.ldo + k;
+        for (int c = 0; c < columns; c += 32) {
+          uint32_t r[32];
+          if (empty) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = 0u;
-        } else {
-          tmem_ld32(taddr + c, r);
-          wait_loaded(r);
-        }
-        const int left = in ? columns - c - lane_row : 0;      // rows from this lane's first on
-        if constexpr (F32OUT) {
+            for (int i = 0; i < 32; ++i) r[i] = 0u;
+          } else {
+            tmem_ld32(taddr + c, r);
+            wait_loaded(r);
+          }
+          const int left = k < g.k ? columns - c : 0;
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             if (i < left) *dst = __uint_as_float(r[i]);
             dst += g.ldo;
           }
-        } else {
-          uint4 v[4];
-          transpose_chunk<BF16>(r, lane, v);
+          if (paced) __nanosleep(kWPause / 2);
+        }
+      } else {
+        // after the exchange a lane has values k .. k + 7 of the rows n, n + 1, ... n + 7
+        const int columns = min(kWTile, g.k - k0), n = n0 + lanes_at + (lane & ~7), k = 8 * (lane & 7), left = g.n - n;
+        uint16_t* dst = static_cast<uint16_t*>(g.out) + e * g.lde + n * g.ldo + k0 + k;
+        for (int c = 0; c < columns; c += 64) {
+          uint4 v[8];
+          if (empty) {
 #pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            if (8 * m < left) *reinterpret_cast<uint4*>(dst) = v[m];
-            dst += row8;
+            for (int i = 0; i < 8; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+          } else {
+            load_row<BF16>(taddr + c, v);
+            transpose_lines(v, lane);
           }
+          if (c + k < columns) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (i < left) *reinterpret_cast<uint4*>(dst + i * g.ldo) = v[i];
+          }
+          dst += 64;
+          if (paced) __nanosleep(kWPause);
         }
       }
       if (!empty) {
@@ -308,7 +360,7 @@ cudaError_t launch(const CUtensorMap& map_dy, const CUtensorMap& map_x, const Wg
     if (clusters <= 0) return cudaErrorLaunchOutOfResources;
     cached[dev] = clusters;
   }
-  return launch_pairs_threads(kernel, kWSmem, tiles < cached[dev] ? tiles : cached[dev], kWThreads, stream, map_dy, map_x, g);
+  return launch_pairs_threads(kernel, kWSmem, tiles < cached[dev] ? tiles : cached[dev], kWThreads, stream, F32OUT ? map_x : map_dy, F32OUT ? map_dy : map_x, g);
 }
 
 }  // namespace
