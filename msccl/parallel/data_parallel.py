@@ -43,13 +43,19 @@ class FlatGradients:
         for flat, _ in self.buckets:
             flat.zero_()
 
+    def _check_views(self):
+        """Every gradient is still its slot of a bucket: what is done to the buckets would pass a replaced one by."""
+        for flat, plan in self.buckets:
+            base, esize = flat.data_ptr(), flat.element_size()
+            for p, off, _ in plan:
+                if p.grad is None or p.grad.data_ptr() != base + off * esize:
+                    raise RuntimeError('a gradient was replaced; keep optimizer.zero_grad(set_to_none=False)')
+
     def all_reduce_gradients(self, all_reduce, world, average=True):
         """Sum every bucket over the ranks with ``all_reduce(flat)`` (for example ``executor.all_reduce``) and,
         with ``average``, divide by ``world``."""
-        for flat, plan in self.buckets:
-            for p, off, n in plan:
-                if p.grad is None or p.grad.data_ptr() != flat[off:off + n].data_ptr():
-                    raise RuntimeError('a gradient was replaced; keep optimizer.zero_grad(set_to_none=False)')
+        self._check_views()
+        for flat, _ in self.buckets:
             all_reduce(flat)
             if average:
                 flat.div_(world)
@@ -57,5 +63,6 @@ class FlatGradients:
     def clip_grad_norm(self, max_norm, reduce=None):
         """Scale all gradients by ``min(1, max_norm / (norm + 1e-6))`` in place, ``norm`` their global 2-norm, and return it
         (``msccl.ops.grad_norm.clip_grad_norm`` on the buckets; the slots' padding is zero).  After ``all_reduce_gradients`` every rank
-        has the same gradients and needs no ``reduce``."""
+        has the same gradients and needs no ``reduce``.  Like that method it raises ``RuntimeError`` where a gradient was replaced."""
+        self._check_views()
         return clip_grad_norm([flat for flat, _ in self.buckets], max_norm, reduce=reduce)
