@@ -47,8 +47,8 @@ class FlatGradients:
         """Every gradient is still its slot of a bucket: what is done to the buckets would pass a replaced one by."""
         for flat, plan in self.buckets:
             base, esize = flat.data_ptr(), flat.element_size()
-            for p, off, _ in plan:
-                if p.grad is None or p.grad.data_ptr() != base + off * esize:
+            for p, off, n in plan:                         # (a tensor without elements has no address)
+                if p.grad is None or n and p.grad.data_ptr() != base + off * esize:
                     raise RuntimeError('a gradient was replaced; keep optimizer.zero_grad(set_to_none=False)')
 
     def all_reduce_gradients(self, all_reduce, world, average=True):

@@ -47,3 +47,12 @@ def test_a_replaced_gradient_is_refused(model, which):
     with pytest.raises(RuntimeError, match='replaced'):
         flat.all_reduce_gradients(calls.append, 2)
     assert not calls, 'a bucket was summed before the gradients of a later one were looked at'
+
+
+def test_a_parameter_without_elements(monkeypatch):
+    monkeypatch.setattr(data_parallel, 'clip_grad_norm', _plain_clip)
+    params = [torch.nn.Parameter(torch.ones(n)) for n in (4, 0, 4)]
+    flat = FlatGradients(params, lambda n, d: torch.empty(n, dtype=d))
+    _backward(params)
+    assert abs(float(flat.clip_grad_norm(1.0)) - 32 ** 0.5) <= 1e-5
+    flat.all_reduce_gradients(lambda t: None, 1)
