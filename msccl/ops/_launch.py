@@ -6,6 +6,7 @@ messages are only put together once one has failed.
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 ELEMS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # ElemType of csrc/expert_ops.h
 
@@ -48,6 +49,16 @@ def stream_handle(index):
 def check(condition, message):
     if not condition:
         raise ValueError(message)
+
+
+def differentiated(a, b=None):
+    """Does autograd follow an operand, backward or forward?  (A tangent is followed without ``requires_grad``, and under ``no_grad`` too.)
+    The operators have backward rules only: their autograd functions then raise ``NotImplementedError``."""
+    if torch.is_grad_enabled() and (a.requires_grad or (b is not None and b.requires_grad)):
+        return True
+    if getattr(forward_ad, '_current_level', 0) < 0:        # no forward mode is active: the usual case, for the price of a comparison
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (a, b))
 
 
 def check_matrix(t, name, dtypes, unit):

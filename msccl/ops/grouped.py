@@ -10,8 +10,8 @@ import torch
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
-from msccl.ops._launch import (ELEMS, check, check_apart, check_devices, check_matrices, check_matrix, check_offsets, check_sizes, error_words,
-                               matrix_stride, on_stream, pitch, stream_handle)
+from msccl.ops._launch import (ELEMS, check, check_apart, check_devices, check_matrices, check_matrix, check_offsets, check_sizes, differentiated,
+                               error_words, matrix_stride, on_stream, pitch, stream_handle)
 from msccl.ops.moe_rows import MAX_EXPERTS, _kernel_rows
 from msccl.runtime.native import load
 
@@ -109,7 +109,7 @@ def grouped_gemm(x, w, offsets, out=None, stream=None):
     n and k multiples of 8, rows contiguous), result [rows, n] of the same type, fp32 sums.  Differentiable in ``x`` and ``w``; with
     ``out`` the result has no gradient."""
     known = _checked(x, 'x', w, offsets, out, False)
-    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+    if differentiated(x, w):
         check(out is None, 'a result written to out has no gradient: detach x and w, or leave out away')
         with on_stream(known[2], stream, (x, w, offsets)):
             return _Grouped.apply(x, w, offsets)

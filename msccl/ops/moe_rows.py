@@ -12,7 +12,7 @@ from typing import NamedTuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from msccl.ops._launch import ELEMS, check_devices, check_matrix, on_stream, pitch, stream_handle
+from msccl.ops._launch import ELEMS, check_devices, check_matrix, differentiated, on_stream, pitch, stream_handle
 from msccl.runtime.native import load
 
 MAX_EXPERTS, MAX_TOPK, MAX_COPIES = 512, 8, 1 << 22
@@ -130,7 +130,7 @@ def gather_rows(x, order, stream=None):
     if x.shape[0] != tokens:
         raise ValueError(f'x has {x.shape[0]} rows, the order {tokens} tokens')
     with on_stream(check_devices('x order', x, order.position), stream, (x, order.position)):
-        return _Gather.apply(x, order) if torch.is_grad_enabled() and x.requires_grad else _scatter(x, order)
+        return _Gather.apply(x, order) if differentiated(x) else _scatter(x, order)
 
 
 def combine_rows(ys, weights, order, stream=None):
@@ -145,5 +145,4 @@ def combine_rows(ys, weights, order, stream=None):
         raise ValueError(f'weights must be a [{tokens}, {topk}] float32 tensor')
     with on_stream(check_devices('ys weights order', ys, weights, order.position), stream, (ys, weights, order.position)):
         weights = weights.contiguous()
-        needs = torch.is_grad_enabled() and (ys.requires_grad or weights.requires_grad)
-        return _Combine.apply(ys, weights, order) if needs else _combine(ys, weights, order)
+        return _Combine.apply(ys, weights, order) if differentiated(ys, weights) else _combine(ys, weights, order)
