@@ -7,6 +7,9 @@
 //   combine   y[t] = sum_j w[t, j] ys[position[t, j]]           (dropped copies contribute nothing and are not read)
 //   backward  of scatter: combine with w = 1; of combine: dys[position[t, j]] = w[t, j] dy[t], dw[t, j] = <dy[t], ys[position[t, j]]>.
 //
+// Positions and the number of kept rows come from the device and may be anything: a row outside [0, tokens * topk) is neither read nor
+// written.
+//
 // All four are memory bound.  One CTA takes one token, so that a row of x (of dy) is read once and written topk times, where a
 // CTA per copy would read it topk times; sums over j and over the row stay in fp32 registers and have one fixed order.
 #include <cuda_bf16.h>
@@ -27,6 +30,7 @@ constexpr int kSortThreads = 1024;             // copies per CTA
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortMaxExperts = 512;
 constexpr int kRowsMaxTopk = 8;
+constexpr long long kMaxCopies = 1 << 22;
 constexpr int kRowThreads = 256;
 
 // Every CTA orders its own 1024 copies.  It needs the expert counts of all copies and of the copies before its own.  Up to 32 CTAs
@@ -183,6 +187,12 @@ template <> struct Pack<__half> {
   }
 };
 
+// The row of copy j of this CTA's token, or -1.
+__device__ __forceinline__ int row_of(const int* __restrict__ position, int topk, int j) {
+  if (j >= topk) return -1;
+  const int row = position[static_cast<long long>(blockIdx.x) * topk + j];
+  return static_cast<unsigned int>(row) < gridDim.x * static_cast<unsigned int>(topk) ? row : -1;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
@@ -192,13 +202,13 @@ scatter_rows_kernel(const T* __restrict__ x, long long ldx, T* __restrict__ out,
   const int kept = *rows_kept, vecs = hidden / Pack<T>::kN;
   int rows[kRowsMaxTopk];
 #pragma unroll
-  for (int j = 0; j < kRowsMaxTopk; ++j) rows[j] = j < topk ? position[t * topk + j] : 0;
+  for (int j = 0; j < kRowsMaxTopk; ++j) rows[j] = row_of(position, topk, j);
   const uint4* src = reinterpret_cast<const uint4*>(x + t * ldx);
   for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
     const uint4 val = src[v];
 #pragma unroll
     for (int j = 0; j < kRowsMaxTopk; ++j)
-      if (j < topk)
+      if (rows[j] >= 0)
         reinterpret_cast<uint4*>(out + static_cast<long long>(rows[j]) * hidden)[v] = rows[j] < kept ? val : make_uint4(0, 0, 0, 0);
   }
 }
@@ -216,7 +226,8 @@ combine_rows_kernel(const T* __restrict__ ys, long long ldy, const float* __rest
   float w[K];
 #pragma unroll
   for (int j = 0; j < K; ++j) {
-    rows[j] = j < topk ? position[t * topk + j] : kept;
+    rows[j] = row_of(position, topk, j);
+    if (rows[j] >= kept) rows[j] = -1;
     w[j] = WEIGHTED && j < topk ? weights[t * topk + j] : 1.0f;
   }
   for (int v0 = threadIdx.x; v0 < vecs; v0 += V * blockDim.x) {
@@ -225,7 +236,7 @@ combine_rows_kernel(const T* __restrict__ ys, long long ldy, const float* __rest
     for (int i = 0; i < V; ++i)
 #pragma unroll
       for (int j = 0; j < K; ++j)
-        if (rows[j] < kept && v0 + i * blockDim.x < vecs)
+        if (rows[j] >= 0 && v0 + i * blockDim.x < vecs)
           val[i][j] = reinterpret_cast<const uint4*>(ys + static_cast<long long>(rows[j]) * ldy)[v0 + i * blockDim.x];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -235,7 +246,7 @@ combine_rows_kernel(const T* __restrict__ ys, long long ldy, const float* __rest
       for (int c = 0; c < N; ++c) sum[c] = 0.0f;
 #pragma unroll
       for (int j = 0; j < K; ++j)
-        if (rows[j] < kept) {
+        if (rows[j] >= 0) {
           float f[N];
           Pack<T>::load(val[i][j], f);
 #pragma unroll
@@ -259,7 +270,7 @@ combine_backward_kernel(const T* __restrict__ dy, long long lddy, const T* __res
   float w[K], dot[K];
 #pragma unroll
   for (int j = 0; j < K; ++j) {
-    rows[j] = j < topk ? position[t * topk + j] : kept;
+    rows[j] = row_of(position, topk, j);
     w[j] = j < topk ? weights[t * topk + j] : 0.0f;
     dot[j] = 0.0f;
   }
@@ -273,7 +284,7 @@ combine_backward_kernel(const T* __restrict__ dy, long long lddy, const T* __res
       gv[i] = src[v];
 #pragma unroll
       for (int j = 0; j < K; ++j)
-        if (rows[j] < kept && dweights != nullptr) val[i][j] = reinterpret_cast<const uint4*>(ys + static_cast<long long>(rows[j]) * ldy)[v];
+        if (rows[j] >= 0 && rows[j] < kept && dweights != nullptr) val[i][j] = reinterpret_cast<const uint4*>(ys + static_cast<long long>(rows[j]) * ldy)[v];
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -283,7 +294,7 @@ combine_backward_kernel(const T* __restrict__ dy, long long lddy, const T* __res
       Pack<T>::load(gv[i], g);
 #pragma unroll
       for (int j = 0; j < K; ++j) {
-        if (j >= topk) continue;
+        if (rows[j] < 0) continue;
         float f[N];
         if (rows[j] < kept) {
           if (dweights != nullptr) {
@@ -319,7 +330,7 @@ combine_backward_kernel(const T* __restrict__ dy, long long lddy, const T* __res
 
 bool rows_ok(int tokens, int topk, int hidden, int elem) {
   const int n = elem == kElemF32 ? 4 : 8;
-  return tokens >= 1 && topk >= 1 && topk <= kRowsMaxTopk && hidden >= n && hidden % n == 0;
+  return tokens >= 1 && topk >= 1 && topk <= kRowsMaxTopk && static_cast<long long>(tokens) * topk <= kMaxCopies && hidden >= n && hidden % n == 0;
 }
 
 // One thread per 16 bytes of a row, whole warps, at most kRowThreads.
@@ -340,7 +351,7 @@ long long sort_copies_workspace(long long n, int experts) {
 // expert_of: n ids (int32, or int64 with wide_ids).
 cudaError_t launch_sort_copies(const void* expert_of, bool wide_ids, long long n, int experts, int* sorted_copy, int* expert_start,
                                int* position, int* workspace, cudaStream_t stream) {
-  if (n < 1 || n > (1 << 22) || experts < 1 || experts > kSortMaxExperts) return cudaErrorInvalidValue;
+  if (n < 1 || n > kMaxCopies || experts < 1 || experts > kSortMaxExperts) return cudaErrorInvalidValue;
   const int grid = static_cast<int>((n + kSortThreads - 1) / kSortThreads), count = static_cast<int>(n);
   int* counts = sort_copies_workspace(n, experts) > 0 ? workspace : nullptr;
   auto run = [&](auto* ids) {

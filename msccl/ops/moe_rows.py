@@ -21,7 +21,8 @@ MAX_EXPERTS, MAX_TOPK, MAX_COPIES = 512, 8, 1 << 22
 class CopyOrder(NamedTuple):
     """``sorted_copy`` [tokens * k] int32: copies (``token * k + j``) ordered by expert, equal ones by number, dropped ones last.
     ``offsets`` [num_experts + 1] int32: the rows of each expert; rows from ``offsets[-1]`` on belong to dropped copies.
-    ``position`` [tokens, k] int32: the row of each copy.  The tensors are made by ``sort_copies`` and are not to be changed."""
+    ``position`` [tokens, k] int32: the row of each copy.  The tensors are made by ``sort_copies`` and are not to be changed.
+    (One that was changed gives wrong rows, but none outside the operands is read or written.)"""
     sorted_copy: torch.Tensor
     offsets: torch.Tensor
     position: torch.Tensor
@@ -53,6 +54,19 @@ def sort_copies(experts, num_experts, stream=None):
 
 def _check_rows(t, name):
     check_matrix(t, name, ELEMS, 4 if t.dtype == torch.float32 else 8)
+
+
+def _check_order(order):
+    """Tokens and copies of each."""
+    sorted_copy, offsets, position = order
+    shape, starts = position.shape, offsets.shape
+    if (len(shape) != 2 or len(starts) != 1 or position.dtype != torch.int32 or offsets.dtype != torch.int32 or starts[0] < 2
+            or not 1 <= shape[1] <= MAX_TOPK or not 1 <= shape[0] * shape[1] <= MAX_COPIES
+            or not position.is_contiguous() or not offsets.is_contiguous()):
+        raise ValueError('order must be as sort_copies makes it: contiguous int32 position [tokens, k] and offsets [experts + 1]')
+    if sorted_copy.numel() != shape[0] * shape[1]:
+        raise ValueError(f'order has {sorted_copy.numel()} sorted copies and {shape[0] * shape[1]} positions: a part of an order is none')
+    return shape
 
 
 def _rows_kept(order):
@@ -126,10 +140,11 @@ def gather_rows(x, order, stream=None):
     ``x`` [tokens, hidden] fp32, bf16 or fp16, rows of whole 16-byte units.  The gradient of a token is the sum of its copies'
     (fp32, in the order of ``j``, rounded once)."""
     _check_rows(x, 'x')
-    tokens = order.position.shape[0]
+    tokens, _ = _check_order(order)
     if x.shape[0] != tokens:
         raise ValueError(f'x has {x.shape[0]} rows, the order {tokens} tokens')
-    with on_stream(check_devices('x order', x, order.position), stream, (x, order.position)):
+    index = check_devices('x order.position order.offsets', x, order.position, order.offsets)
+    with on_stream(index, stream, (x, order.position, order.offsets)):
         return _Gather.apply(x, order) if differentiated(x) else _scatter(x, order)
 
 
@@ -138,11 +153,12 @@ def combine_rows(ys, weights, order, stream=None):
     fp32 sums in the order of ``j``, rounded once.  ``ys`` [tokens * k, hidden] fp32, bf16 or fp16, ``weights`` [tokens, k] fp32.
     Gradients: ``ys`` and ``weights`` (zero for dropped copies)."""
     _check_rows(ys, 'ys')
-    tokens, topk = order.position.shape
+    tokens, topk = _check_order(order)
     if ys.shape[0] != tokens * topk:
         raise ValueError(f'ys has {ys.shape[0]} rows, the order {tokens * topk} copies')
     if weights.dtype != torch.float32 or weights.shape != (tokens, topk):
         raise ValueError(f'weights must be a [{tokens}, {topk}] float32 tensor')
-    with on_stream(check_devices('ys weights order', ys, weights, order.position), stream, (ys, weights, order.position)):
+    index = check_devices('ys weights order.position order.offsets', ys, weights, order.position, order.offsets)
+    with on_stream(index, stream, (ys, weights, order.position, order.offsets)):
         weights = weights.contiguous()
         return _Combine.apply(ys, weights, order) if differentiated(ys, weights) else _combine(ys, weights, order)
