@@ -90,10 +90,11 @@ def _combine(ys, weights, order):
 
 
 def _kernel_rows(g, like):
-    """An incoming gradient as the kernels take it: autograd may hand over an expanded or otherwise strided tensor."""
+    """An incoming gradient as the kernels take it (``check_matrix``): autograd may hand over an expanded or otherwise strided tensor,
+    rows that overlap among them."""
     g = g.to(like)
     unit = 16 // g.element_size()
-    if g.stride(-1) != 1 or g.data_ptr() % 16 or (g.shape[0] > 1 and (g.stride(0) % unit or g.stride(0) <= 0)):
+    if g.stride(-1) != 1 or g.data_ptr() % 16 or (g.shape[0] > 1 and (g.stride(0) % unit or g.stride(0) < g.shape[1])):
         g = g.contiguous()
     return g.clone() if g.data_ptr() % 16 else g
 
