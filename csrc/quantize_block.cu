@@ -59,6 +59,12 @@ __device__ __forceinline__ float block_scale(uint32_t bits) {
   const float floor_value = 0x1p-100f;
   return __fdiv_rn(__uint_as_float(max(bits, __float_as_uint(floor_value))), 448.0f);
 }
+__device__ __forceinline__ uint2 to_e4m3(const float (&v)[8]) {
+  uint32_t p[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(p[0] | p[1] << 16, p[2] | p[3] << 16);
+}
 // x / scale, correctly rounded: the quotient from the correctly rounded reciprocal, corrected once by its exact remainder (Markstein,
 // "Computation of elementary functions on the IBM RISC System/6000 processor", 1990, theorem on division).  Scales are between
 // 2^-109 and 2^120, so the reciprocal is a normal number.  The remainder is a multiple of more than 2^-48 |q| scale and has to be one of
@@ -66,12 +72,6 @@ __device__ __forceinline__ float block_scale(uint32_t bits) {
 // and x with them, which is exact (without that, blocks whose largest magnitude is near 2^-99 had bytes off by one at ties).  In every thread:
 // 8192 x 14336 takes 95 us instead of 91, with a branch around it 93, or 97 where it is taken.  An infinite
 // or NaN scale takes the division itself.  Eight divisions per thread made the kernel slower than memory (8192 x 14336: 123 us).
-__device__ __forceinline__ uint2 to_e4m3(const float (&v)[8]) {
-  uint32_t p[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) p[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-  return make_uint2(p[0] | p[1] << 16, p[2] | p[3] << 16);
-}
 __device__ __forceinline__ uint2 quantize8(const float (&v)[8], float scale) {
   float q[8];
   if (scale < INFINITY) {
@@ -80,7 +80,7 @@ __device__ __forceinline__ uint2 quantize8(const float (&v)[8], float scale) {
     for (int i = 0; i < 8; ++i) {
       const float x = v[i] * lift;
       q[i] = x * reciprocal;
-      q[i] = fmaf(fmaf(-q[i], divisor, x), reciprocal, q[i]);
+      q[i] = fmaf(fmaf(q[i], divisor, -x), -reciprocal, q[i]);      // the remainder negated: a zero keeps its sign this way
     }
   } else {
 #pragma unroll
