@@ -148,8 +148,20 @@ __global__ void __launch_bounds__(kGradThreads) grad_sum_kernel(const double* __
   }
 }
 
+// A factor below 2^-126 (gradients of 1e37) has few bits or none in fp32 although its products may be ordinary numbers.  So it
+// comes in two parts: a power of two and the rest.  The first is 1 for all others, and where it is not, what a multiplication by it
+// may round is far below the least product that fp32 holds.
+struct Factor {
+  float power, rest;
+  __device__ __forceinline__ explicit Factor(double ratio) {
+    power = ratio >= 0x1p-126 || !(ratio > 0.0) ? 1.0f : ratio >= 0x1p-190 ? 0x1p-64f : 0x1p-126f;
+    rest = ratio > 1.0 ? 1.0f : static_cast<float>(ratio / power);            // a NaN stays one
+  }
+  __device__ __forceinline__ float operator*(float v) const { return v * power * rest; }
+};
+
 template <typename S, typename D>
-__device__ __forceinline__ void chunk_scale(const S* src, D* dst, int n, float factor) {
+__device__ __forceinline__ void chunk_scale(const S* src, D* dst, int n, Factor factor) {
   // The wider of the two types moves 16 bytes per lane, so that every access of a warp is one stretch of memory (8 elements a lane
   // would write fp32 as two halves of a 32-byte sector at different times: 256 Mi bf16 -> fp32 356 us, now 270).  Element by
   // element where the two sides cannot be aligned together.
@@ -158,7 +170,7 @@ __device__ __forceinline__ void chunk_scale(const S* src, D* dst, int n, float f
   int head = static_cast<int>((as - reinterpret_cast<uintptr_t>(src) % as) % as / sizeof(S));
   if (reinterpret_cast<uintptr_t>(dst + head) % ad != 0) head = n;
   head = min(head, n);
-  for (int i = threadIdx.x; i < head; i += kGradThreads) dst[i] = from_f32<D>(to_f32(src[i]) * factor);
+  for (int i = threadIdx.x; i < head; i += kGradThreads) dst[i] = from_f32<D>(factor * to_f32(src[i]));
   const int vecs = (n - head) / N;
   const Vec<S, N>* sv = reinterpret_cast<const Vec<S, N>*>(src + head);
   Vec<D, N>* dv = reinterpret_cast<Vec<D, N>*>(dst + head);
@@ -171,7 +183,7 @@ __device__ __forceinline__ void chunk_scale(const S* src, D* dst, int n, float f
     for (int u = 0; u < U; ++u) {
       Vec<D, N> y;
 #pragma unroll
-      for (int e = 0; e < N; ++e) y.v[e] = from_f32<D>(to_f32(x[u].v[e]) * factor);
+      for (int e = 0; e < N; ++e) y.v[e] = from_f32<D>(factor * to_f32(x[u].v[e]));
       dv[i + u * kGradThreads] = y;
     }
   }
@@ -179,14 +191,14 @@ __device__ __forceinline__ void chunk_scale(const S* src, D* dst, int n, float f
     const Vec<S, N> x = sv[i];
     Vec<D, N> y;
 #pragma unroll
-    for (int e = 0; e < N; ++e) y.v[e] = from_f32<D>(to_f32(x.v[e]) * factor);
+    for (int e = 0; e < N; ++e) y.v[e] = from_f32<D>(factor * to_f32(x.v[e]));
     dv[i] = y;
   }
-  for (int t = head + vecs * N + threadIdx.x; t < n; t += kGradThreads) dst[t] = from_f32<D>(to_f32(src[t]) * factor);
+  for (int t = head + vecs * N + threadIdx.x; t < n; t += kGradThreads) dst[t] = from_f32<D>(factor * to_f32(src[t]));
 }
 
 template <typename S>
-__device__ __forceinline__ void chunk_scale_to(const GradTensor& t, long long lo, int n, float factor) {
+__device__ __forceinline__ void chunk_scale_to(const GradTensor& t, long long lo, int n, Factor factor) {
   const S* src = static_cast<const S*>(t.src) + lo;
   if (t.dst_type == kElemF32) chunk_scale(src, static_cast<float*>(t.dst) + lo, n, factor);
   else if (t.dst_type == kElemBF16) chunk_scale(src, static_cast<__nv_bfloat16*>(t.dst) + lo, n, factor);
@@ -194,16 +206,15 @@ __device__ __forceinline__ void chunk_scale_to(const GradTensor& t, long long lo
 }
 
 template <int MAX>
-__global__ void __launch_bounds__(kGradThreads)
+__global__ void __launch_bounds__(kGradThreads, 5)           // at most 48 registers: with 50 (four CTAs) those 275 us are 287
 grad_scale_kernel(const __grid_constant__ GradList<MAX> list, const double* __restrict__ partials, int partial_count, double max_norm,
                   float* __restrict__ norm_out) {
   const double norm = sqrt(sum_partials(partials, partial_count));
   if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out != nullptr) *norm_out = static_cast<float>(norm);
-  const double ratio = max_norm / (norm + 1e-6);
-  const float factor = ratio > 1.0 ? 1.0f : static_cast<float>(ratio);        // a NaN stays one
+  const Factor factor(max_norm / (norm + 1e-6));
   for (int c = blockIdx.x; c < list.chunks; c += gridDim.x) {
     const GradTensor& t = list.t[find_tensor(list, c)];
-    if (factor == 1.0f && t.src == t.dst) continue;
+    if (factor.rest == 1.0f && factor.power == 1.0f && t.src == t.dst) continue;
     const long long lo = static_cast<long long>(c - t.first_chunk) * kChunk;
     const int n = static_cast<int>(min(static_cast<long long>(kChunk), t.numel - lo));
     if (t.src_type == kElemF32) chunk_scale_to<float>(t, lo, n, factor);
