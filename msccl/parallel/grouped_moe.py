@@ -16,7 +16,8 @@ class GroupedMoE(torch.nn.Module):
 
     ``forward`` takes any number of tokens (one at least), [tokens, hidden] in the layer's dtype, and is differentiable in ``x``, the
     router and the experts.  ``quantize()`` makes the fp8 form of the experts (of a bf16 layer); ``forward(x, precision='fp8')`` then runs
-    on it, without gradients; the default runs in the layer's own type.  hidden and ffn: multiples of 8 (16 for fp8)."""
+    on it, without gradients; the default runs in the layer's own type.  The fp8 form moves with the layer to another device; loading a state
+    or changing the layer's type ends it, until the next ``quantize()``.  hidden and ffn: multiples of 8 (16 for fp8)."""
 
     def __init__(self, hidden, ffn, num_experts, topk=2, device='cuda', dtype=torch.bfloat16, std=0.02, seed=0):
         super().__init__()
@@ -36,6 +37,19 @@ class GroupedMoE(torch.nn.Module):
             raise ValueError(f'the fp8 products give bf16, the layer is {self.w_down.dtype}')
         self._fp8 = quantize_fp8_block_weight(self.w_gate_up.detach()) + quantize_fp8_block_weight(self.w_down.detach())
         return self
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        if self._fp8 is not None:
+            # fn moves tensors and converts floating-point ones: as integers these keep their bits
+            moved = [(fn(t.view(bits)), bits, t.dtype) for t, bits in zip(self._fp8, (torch.uint8, torch.int32) * 2)]
+            kept = self.w_down.dtype == torch.bfloat16 and all(m.dtype == bits for m, bits, _ in moved)
+            self._fp8 = tuple(m.view(dtype) for m, _, dtype in moved) if kept else None
+        return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        self._fp8 = None                                     # of the weights that were there before
+        super()._load_from_state_dict(*args, **kwargs)
 
     def _experts(self, xs, offsets):
         gate, up = grouped_gemm(xs, self.w_gate_up, offsets).split(self.ffn, 1)
