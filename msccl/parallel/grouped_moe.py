@@ -7,7 +7,7 @@ import torch
 from msccl.ops.fp8_block import grouped_gemm_fp8_block, quantize_fp8_block, quantize_fp8_block_weight
 from msccl.ops.grouped import grouped_gemm
 from msccl.ops.moe import route_top_k
-from msccl.ops.moe_rows import combine_rows, gather_rows, sort_copies
+from msccl.ops.moe_rows import MAX_EXPERTS, MAX_TOPK, combine_rows, gather_rows, sort_copies
 
 
 class GroupedMoE(torch.nn.Module):
@@ -21,6 +21,13 @@ class GroupedMoE(torch.nn.Module):
 
     def __init__(self, hidden, ffn, num_experts, topk=2, device='cuda', dtype=torch.bfloat16, std=0.02, seed=0):
         super().__init__()
+        if not 1 <= num_experts <= MAX_EXPERTS:
+            raise ValueError(f'between 1 and {MAX_EXPERTS} experts are supported (got {num_experts})')
+        if not 1 <= topk <= min(MAX_TOPK, num_experts):
+            raise ValueError(f'topk must be within 1 and {min(MAX_TOPK, num_experts)} with {num_experts} experts (got {topk})')
+        for name, size in (('hidden', hidden), ('ffn', ffn)):
+            if size < 8 or size % 8:
+                raise ValueError(f'{name} must be a positive multiple of 8 (got {size})')
         self.hidden, self.ffn, self.num_experts, self.topk = hidden, ffn, num_experts, topk
         gen = torch.Generator(device=device).manual_seed(seed)
 
