@@ -20,6 +20,9 @@ def _errors(device):
     key = torch.device(device).index or 0
     if key not in _error_words:
         _error_words[key] = torch.zeros(4, dtype=torch.int32, device=f'cuda:{key}')
+        if not torch.cuda.is_current_stream_capturing():
+            # kernels of any stream read them, and what they held before they were cleared would look like a report
+            torch.cuda.current_stream(key).synchronize()
     return _error_words[key]
 
 
