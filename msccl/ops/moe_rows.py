@@ -46,9 +46,9 @@ def sort_copies(experts, num_experts, stream=None):
         workspace = native.sort_copies_workspace(copies, num_experts) if copies > 1024 else 0
         table = torch.empty(2 * copies + num_experts + 1, dtype=torch.int32, device=experts.device)
         sorted_copy, position, offsets = table.split((copies, copies, num_experts + 1))
-        counts = torch.empty(workspace, dtype=torch.int32, device=experts.device).data_ptr() if workspace else 0
+        counts = torch.empty(workspace, dtype=torch.int32, device=experts.device) if workspace else None     # alive until the launch
         native.sort_copies(experts.data_ptr(), experts.dtype == torch.int64, copies, num_experts, sorted_copy.data_ptr(),
-                           offsets.data_ptr(), position.data_ptr(), counts, stream_handle(index))
+                           offsets.data_ptr(), position.data_ptr(), 0 if counts is None else counts.data_ptr(), stream_handle(index))
     return CopyOrder(sorted_copy, offsets, position.view(tokens, topk))
 
 
