@@ -16,8 +16,11 @@
 // 614 us), CTA pairs with 256 x 256 (481: one block per accumulator) and 256 x 128 tiles (438, and 549 against 519 us at 8192 x 14336 x
 // 4096).
 //
-// With at most 32 rows in all only 32 rows of `a` are loaded; the tensor core then reads whatever follows in shared memory as
-// the other rows (still inside the allocation) and their results are not read.
+// With at most 32 rows in all only 32 rows of `a` are loaded; the tensor core then reads what follows in the same stage as the
+// other rows, and their results are not read.
+//
+// The two scales of a block are multiplied with each other in fp32, so that product has to be a normal number (as those of
+// quantize_block.cu's scales are, unless both operands are near an end of fp32's range).
 //
 // Every wait is bounded (gemm_sm100.cuh).
 #include <cuda.h>
@@ -184,12 +187,12 @@ template <int BN, int AR> struct FGeometry {
   static constexpr int kABytes = AR * kFBlock;
   static constexpr int kBBytes = BN * kFBlock;
   static constexpr int kStageBytes = kU * (kABytes + kBBytes);        // kU blocks of a, then kU blocks of w
-  static constexpr int kBehind = (BM - AR) * kFBlock;       // what the MMA may read behind the last stage
-  static constexpr int kFit = (kFSmemLimit - kBehind) / kStageBytes;
+  static_assert((kU - 1) * kABytes + BM * kFBlock <= kStageBytes, "the MMA reads BM rows of every block of a");
+  static constexpr int kFit = kFSmemLimit / kStageBytes;
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static constexpr int kAccs = 512 / (kU * BN) < 4 ? 512 / (kU * BN) : 4;
   static constexpr int kTmemCols = kAccs * kU * BN;
-  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStageBytes + kBehind + 512;
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStageBytes + 512;
 };
 
 __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
@@ -211,7 +214,7 @@ fp8_block_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   extern __shared__ uint8_t smem_raw[];
   __shared__ GroupTable table;
   uint8_t* stage_base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(stage_base + static_cast<size_t>(S) * Geo::kStageBytes + Geo::kBehind);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(stage_base + static_cast<size_t>(S) * Geo::kStageBytes);
   uint64_t *full_bar = bars, *empty_bar = bars + S, *acc_full = bars + 2 * S, *acc_empty = bars + 2 * S + ACCS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 2 * ACCS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);

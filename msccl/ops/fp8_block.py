@@ -7,7 +7,8 @@ weight (``csrc/fp8_block_gemm.cu``, ``csrc/quantize_block.cu``).  Weights are qu
     y = grouped_gemm_fp8_block(xq, xs, wq, ws, offsets)   # rows of expert e: offsets[e] .. offsets[e + 1]
 
 Beside the MX format of ``msccl.ops.gemm`` (a power of two per 32 values, applied inside the tensor core) these scales are any
-fp32 numbers, the form in which block-quantised checkpoints come.  There are no gradients: this is the path for serving.
+fp32 numbers, the form in which block-quantised checkpoints come.  (The scales of an activation and of a weight are multiplied with each
+other first: that product has to be a normal fp32 number.)  There are no gradients: this is the path for serving.
 """
 import torch
 from torch.autograd.graph import increment_version

@@ -60,7 +60,7 @@ def clip_grad_norm(gradients, max_norm, out=None, reduce=None, stream=None):
     bf16 gradients of a step into the fp32 ones of the optimizer).  In place nothing is written on a step that needs no clipping.
     ``reduce(t)`` sums the one-element float64 tensor ``t`` (this process's sum of squares) over the processes that hold the other
     parts of the gradients, in place; gradients that are the same on every rank need none.  An infinite norm gives zeros (and NaN
-    where the gradient is infinite), a NaN gives NaN everywhere.  No tensor may share memory with another one that is written.
+    where the gradient is infinite; NaN everywhere if ``max_norm`` is infinite too), a NaN gives NaN everywhere.  No tensor may share memory with another one that is written.
     For autograd this is a write under ``no_grad``: a backward pass that needs a written tensor as it was raises."""
     max_norm = float(max_norm)
     check(not math.isnan(max_norm) and max_norm >= 0, f'max_norm must not be negative or NaN (got {max_norm})')

@@ -29,7 +29,8 @@ class CopyOrder(NamedTuple):
 
 
 def sort_copies(experts, num_experts, stream=None):
-    """Stable order of the copies ``experts`` [tokens, k] (int32 or int64) by expert, in one launch (two from 32768 copies on).  A copy whose id is outside
+    """Stable order of the copies ``experts`` [tokens, k] (int32 or int64) by expert, in one launch (two
+    with more than 32768 copies).  A copy whose id is outside
     ``[0, num_experts)`` is dropped: the gather gives it a row of zeros behind the last expert's, the combination ignores it."""
     if experts.dim() != 2 or experts.dtype not in (torch.int32, torch.int64):
         raise ValueError('experts must be a [tokens, k] int32 or int64 tensor')
