@@ -76,9 +76,9 @@ class _Grouped(torch.autograd.Function):
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
         with on_stream(dy.get_device(), None):
-            dy = _kernel_rows(dy, x.dtype)
-            dx = _product(dy, w, offsets, True) if ctx.needs_input_grad[0] else None
-            dw = _weight_gradient(dy, x, offsets) if ctx.needs_input_grad[1] else None
+            dy, offsets = _kernel_rows(dy, x.dtype), offsets.contiguous()
+            dx = _product(dy, _kernel_rows(w, x.dtype), offsets, True) if ctx.needs_input_grad[0] else None
+            dw = _weight_gradient(dy, _kernel_rows(x, x.dtype), offsets) if ctx.needs_input_grad[1] else None
         return dx, dw, None
 
 

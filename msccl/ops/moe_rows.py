@@ -90,14 +90,23 @@ def _combine(ys, weights, order):
     return out
 
 
-def _kernel_rows(g, like):
-    """An incoming gradient as the kernels take it (``check_matrix``): autograd may hand over an expanded or otherwise strided tensor,
-    rows that overlap among them."""
-    g = g.to(like)
-    unit = 16 // g.element_size()
-    if g.stride(-1) != 1 or g.data_ptr() % 16 or (g.shape[0] > 1 and (g.stride(0) % unit or g.stride(0) < g.shape[1])):
-        g = g.contiguous()
-    return g.clone() if g.data_ptr() % 16 else g
+def _kernel_rows(t, dtype):
+    """``t`` as the kernels take it (``check_matrix``, ``check_matrices``), copied if need be.  An incoming gradient may be an expanded or
+    otherwise strided tensor, with rows that overlap; a saved operand may have been unpacked by a hook into any layout."""
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    if t.is_contiguous() and not t.data_ptr() % 16:          # the usual case; the columns are whole units
+        return t
+    unit = 16 // t.element_size()
+    stride, extent = t.stride(), t.shape[-1]
+    good = stride[-1] == 1
+    for dim in range(t.dim() - 2, -1, -1):
+        step = stride[dim] if t.shape[dim] > 1 else extent
+        good = good and step >= extent and not step % unit
+        extent = (t.shape[dim] - 1) * step + extent
+    if not good:
+        t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
 
 
 class _Gather(torch.autograd.Function):
@@ -127,7 +136,7 @@ class _Combine(torch.autograd.Function):
         order = ctx.order
         tokens, topk = order.position.shape
         with on_stream(dy.get_device(), None):
-            dy = _kernel_rows(dy, ys.dtype)
+            dy, ys, weights = _kernel_rows(dy, ys.dtype), _kernel_rows(ys, ys.dtype), weights.contiguous()
             dys = torch.empty(ys.shape, dtype=ys.dtype, device=ys.device) if ctx.needs_input_grad[0] else None
             dweights = torch.empty(weights.shape, dtype=weights.dtype, device=ys.device) if ctx.needs_input_grad[1] else None
             load().combine_backward(dy.data_ptr(), pitch(dy), ys.data_ptr(), pitch(ys), weights.data_ptr(),
