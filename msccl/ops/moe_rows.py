@@ -16,6 +16,7 @@ from msccl.ops._launch import ELEMS, check_devices, check_matrix, differentiated
 from msccl.runtime.native import load
 
 MAX_EXPERTS, MAX_TOPK, MAX_COPIES = 512, 8, 1 << 22
+_INT32 = torch.int32
 
 
 class CopyOrder(NamedTuple):
@@ -60,14 +61,15 @@ def _check_rows(t, name):
 def _check_order(order):
     """Tokens and copies of each."""
     sorted_copy, offsets, position = order
-    shape, starts = position.shape, offsets.shape
-    if (len(shape) != 2 or len(starts) != 1 or position.dtype != torch.int32 or offsets.dtype != torch.int32 or starts[0] < 2
-            or not 1 <= shape[1] <= MAX_TOPK or not 1 <= shape[0] * shape[1] <= MAX_COPIES
-            or not position.is_contiguous() or not offsets.is_contiguous()):
-        raise ValueError('order must be as sort_copies makes it: contiguous int32 position [tokens, k] and offsets [experts + 1]')
-    if sorted_copy.numel() != shape[0] * shape[1]:
-        raise ValueError(f'order has {sorted_copy.numel()} sorted copies and {shape[0] * shape[1]} positions: a part of an order is none')
-    return shape
+    copies = position.numel()
+    if (position.dim() == 2 and position.dtype == _INT32 and position.is_contiguous() and sorted_copy.numel() == copies and 1 <= copies <= MAX_COPIES
+            and offsets.dim() == 1 and offsets.dtype == _INT32 and offsets.is_contiguous() and offsets.numel() > 1):
+        tokens, topk = position.shape
+        if topk <= MAX_TOPK:
+            return tokens, topk
+    raise ValueError('order must be as sort_copies makes it, and whole: contiguous int32 position [tokens, k] (got '
+                     f'{position.dtype} {list(position.shape)}), {copies} sorted copies (got {sorted_copy.numel()}) and offsets [experts + 1] (got '
+                     f'{offsets.dtype} {list(offsets.shape)})')
 
 
 def _rows_kept(order):
