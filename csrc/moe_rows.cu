@@ -187,6 +187,12 @@ template <> struct Pack<__half> {
   }
 };
 
+// CTAs per SM that the row kernels leave room for: left to itself the compiler keeps more addresses in registers (16384 tokens x 2 copies of
+// 4096 bf16: scatter 70 us at 40 registers, 64 at 32; 4096 x 8: combine 47 at 79, 46 at 64, backward 98 at 90, 89 at 80).
+constexpr int kScatterCtas = 8;
+constexpr int combine_ctas(int k) { return k == 8 ? 4 : 6; }
+constexpr int combine_backward_ctas(int k) { return k == 8 ? 3 : k == 1 ? 6 : 4; }
+
 // The row of copy j of this CTA's token, or -1.
 __device__ __forceinline__ int row_of(const int* __restrict__ position, int topk, int j) {
   if (j >= topk) return -1;
@@ -195,7 +201,7 @@ __device__ __forceinline__ int row_of(const int* __restrict__ position, int topk
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, kScatterCtas)
 scatter_rows_kernel(const T* __restrict__ x, long long ldx, T* __restrict__ out, const int* __restrict__ position,
                     const int* __restrict__ rows_kept, int topk, int hidden) {
   const long long t = blockIdx.x;
@@ -216,7 +222,7 @@ scatter_rows_kernel(const T* __restrict__ x, long long ldx, T* __restrict__ out,
 // K >= topk copies and V vectors of a row per thread and step, K * V loads in flight (one vector of a token with two copies kept HBM at
 // 4.0 TB/s).
 template <typename T, int K, bool WEIGHTED>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, combine_ctas(K))
 combine_rows_kernel(const T* __restrict__ ys, long long ldy, const float* __restrict__ weights, T* __restrict__ out,
                     const int* __restrict__ position, const int* __restrict__ rows_kept, int topk, int hidden) {
   constexpr int N = Pack<T>::kN, V = K <= 2 ? 4 / K : 1;
@@ -258,7 +264,7 @@ combine_rows_kernel(const T* __restrict__ ys, long long ldy, const float* __rest
 }
 
 template <typename T, int K>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, combine_backward_ctas(K))
 combine_backward_kernel(const T* __restrict__ dy, long long lddy, const T* __restrict__ ys, long long ldy, const float* __restrict__ weights,
                         T* __restrict__ dys, float* __restrict__ dweights, const int* __restrict__ position,
                         const int* __restrict__ rows_kept, int topk, int hidden) {
