@@ -6,7 +6,8 @@
 // definition alone.  Infinite values make the scale infinite (the block becomes NaN and zeros), NaN makes the whole block NaN:
 // neither can vanish.  The floor keeps the scale of a block of zeros, or of values below 2^-100, a normal number.
 //
-// Memory bound (5 TB/s): a row's 128 bf16 values are 16 lanes x 16 bytes in, 16 lanes x 8 bytes out.
+// A row's 128 bf16 values are 16 lanes x 16 bytes in, 16 lanes x 8 bytes out.  fp32 is bound by memory (8192 x 14336: 99 us, 5.9 TB/s; a
+// weight of 8 x 14336 x 4096: 327 us, 7.2 TB/s), 16-bit types by the instructions for each value (93 us, 3.8 TB/s; 327 us, 4.3 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -70,8 +71,8 @@ __device__ __forceinline__ uint2 to_e4m3(const float (&v)[8]) {
 // 2^-109 and 2^120, so the reciprocal is a normal number.  The remainder is a multiple of more than 2^-48 |q| scale and has to be one of
 // 2^-149 to be exact; quotients below 2^-11 are zero in e4m3 whatever the last bits are.  So scales below 2^-60 are multiplied by 2^64 first,
 // and x with them, which is exact (without that, blocks whose largest magnitude is near 2^-99 had bytes off by one at ties).  In every thread:
-// 8192 x 14336 takes 95 us instead of 91, with a branch around it 93, or 97 where it is taken.  An infinite
-// or NaN scale takes the division itself.  Eight divisions per thread made the kernel slower than memory (8192 x 14336: 123 us).
+// calls of 8192 x 14336 take 95 us instead of 91, with a branch around it 93, or 97 where it is taken.  An infinite
+// or NaN scale takes the division itself.  Eight divisions per thread took 123 us for 8192 x 14336.
 __device__ __forceinline__ uint2 quantize8(const float (&v)[8], float scale) {
   float q[8];
   if (scale < INFINITY) {

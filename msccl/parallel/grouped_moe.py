@@ -14,7 +14,7 @@ class GroupedMoE(torch.nn.Module):
     """``y[t] = sum_j p[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t]))`` over the ``topk`` experts ``e`` of token ``t``, ``p`` the softmax
     over their router logits.
 
-    ``forward`` takes any number of tokens (one at least), [tokens, hidden] in the layer's dtype, and is differentiable in ``x``, the
+    ``forward`` takes any number of tokens (one at least, at most 2 ** 22 copies of them), [tokens, hidden] in the layer's dtype, and is differentiable in ``x``, the
     router and the experts.  ``quantize()`` makes the fp8 form of the experts (of a bf16 layer); ``forward(x, precision='fp8')`` then runs
     on it, without gradients; the default runs in the layer's own type.  The fp8 form moves with the layer to another device; loading a state
     or changing the layer's type ends it, until the next ``quantize()``.  hidden and ffn: multiples of 8 (16 for fp8)."""
