@@ -19,10 +19,16 @@ class GemmKernelError(RuntimeError):
 def _errors(device):
     key = torch.device(device).index or 0
     if key not in _error_words:
-        _error_words[key] = torch.zeros(4, dtype=torch.int32, device=f'cuda:{key}')
-        if not torch.cuda.is_current_stream_capturing():
-            # kernels of any stream read them, and what they held before they were cleared would look like a report
-            torch.cuda.current_stream(key).synchronize()
+        if torch.cuda.is_current_stream_capturing():
+            _error_words[key] = torch.zeros(4, dtype=torch.int32, device=f'cuda:{key}')
+        else:
+            # Kernels of any stream read them, and what they held before they were cleared would look like a report.  Cleared on a stream of
+            # their own: the current one may hold work that waits for what this thread launches next.
+            clearing = torch.cuda.Stream(key, priority=-1)
+            with torch.cuda.stream(clearing):
+                words = torch.zeros(4, dtype=torch.int32, device=f'cuda:{key}')
+            clearing.synchronize()
+            _error_words[key] = words
     return _error_words[key]
 
 
