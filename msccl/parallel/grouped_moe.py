@@ -54,9 +54,10 @@ class GroupedMoE(torch.nn.Module):
             self._fp8 = tuple(m.view(dtype) for m, _, dtype in moved) if kept else None
         return self
 
-    def _load_from_state_dict(self, *args, **kwargs):
-        self._fp8 = None                                     # of the weights that were there before
-        super()._load_from_state_dict(*args, **kwargs)
+    def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
+        if prefix + 'w_gate_up' in state_dict or prefix + 'w_down' in state_dict:
+            self._fp8 = None                                 # of the weights that were there before
+        super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
 
     def _experts(self, xs, offsets):
         gate, up = grouped_gemm(xs, self.w_gate_up, offsets).split(self.ffn, 1)

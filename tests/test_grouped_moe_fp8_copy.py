@@ -45,6 +45,16 @@ def test_loading_into_a_larger_model_ends_it_too(layer):
         layer(X, precision='fp8')
 
 
+def test_a_state_without_the_experts_leaves_it(layer):
+    before = _bytes(layer)
+    layer.load_state_dict({'w_router': torch.zeros_like(layer.w_router)}, strict=False)
+    model = torch.nn.Sequential(torch.nn.Linear(2, 2), layer)
+    model.load_state_dict({'0.weight': torch.zeros(2, 2), 'w_down': layer.w_down}, strict=False)
+    assert _same(_bytes(layer), before)
+    layer.load_state_dict({'w_down': torch.zeros_like(layer.w_down)}, strict=False)
+    assert layer._fp8 is None
+
+
 def test_a_move_takes_the_copy_along(layer):
     before = _bytes(layer)
     assert _same(_bytes(layer.cpu()), before) and _same(_bytes(layer.to(torch.bfloat16)), before)
