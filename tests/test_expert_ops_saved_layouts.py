@@ -1,6 +1,7 @@
 """What a backward pass reads may come back from a saved-tensor hook with other strides, or off the boundary of 16 bytes: the kernels get
 none of that.  On the CPU, with the launches replaced by checks of their arguments."""
 import contextlib
+import ctypes
 
 import pytest
 import torch
@@ -33,7 +34,7 @@ class _Native:
     def combine_backward(self, dy, lddy, ys, ldy, weights, *rest):
         self.calls.append('combine')
         assert not (dy % 16 or ys % 16 or lddy % UNIT or ldy % UNIT) and self.weights[0].data_ptr() != 0
-        hidden, read = rest[6], torch.frombuffer((__import__('ctypes').c_float * 6).from_address(weights), dtype=torch.float32)
+        hidden, read = rest[6], torch.frombuffer((ctypes.c_float * 6).from_address(weights), dtype=torch.float32)
         assert hidden == 16 and torch.equal(read, self.weights[0].reshape(-1)), 'weights are read as they lie in memory'
 
 
